@@ -8,12 +8,17 @@
 
 #include <atomic>
 
+#include "capi_util.h"
 #include "h3attn.h"
 #include "kernels.h"
 
 namespace {
 
 thread_local char g_err[512] = "";
+
+}  // namespace
+
+namespace h3a {
 
 int fail(int code, const char* fmt, ...) {
     va_list ap;
@@ -22,6 +27,31 @@ int fail(int code, const char* fmt, ...) {
     va_end(ap);
     return code;
 }
+
+void clear_error() { g_err[0] = '\0'; }
+
+int device_cus() {
+    static std::atomic<int> cache[64];
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0) return 0;
+    if (dev < 64) {
+        const int c = cache[dev].load(std::memory_order_relaxed);
+        if (c > 0) return c;
+    }
+    int n = 0;
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess) return 0;
+    if (dev < 64) cache[dev].store(n, std::memory_order_relaxed);
+    return n;
+}
+
+}  // namespace h3a
+
+namespace {
+
+using h3a::aligned16;
+using h3a::aligned4;
+using h3a::device_cus;
+using h3a::fail;
 
 constexpr int64_t kMaxWindow = (int64_t)1 << 31;  // buffer offsets are 32-bit
 // The d-major V copy costs a pass over V (about 25 us at 5 heads x 49,920
@@ -69,9 +99,6 @@ bool short_segments_planned(const h3a_attn_args* a, int cus) {
     if (a->cu_seqlens_k != a->cu_seqlens_q && a->seqlen_k >= kLongKeys) return m.rounds <= 3.2;
     return m.rounds >= 1.0 && m.rounds <= 5.0;
 }
-
-bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
-bool aligned4(const void* p) { return ((uintptr_t)p & 3u) == 0; }
 
 // Validates the arguments and fills the launch description (split off);
 // *empty: nothing to launch.
@@ -166,21 +193,6 @@ int prepare_attn(const h3a_attn_args* a, h3a::AttnParams& p, bool* empty) {
     const int64_t blocks = (int64_t)p.n_qtiles * p.heads * p.n_groups;
     if (blocks > INT32_MAX) return fail(H3A_EUNSUPPORTED, "h3a_attn_fwd: grid too large");
     return H3A_OK;
-}
-
-// CU count of the current device, cached per device.
-int device_cus() {
-    static std::atomic<int> cache[64];
-    int dev = 0;
-    if (hipGetDevice(&dev) != hipSuccess || dev < 0) return 0;
-    if (dev < 64) {
-        const int c = cache[dev].load(std::memory_order_relaxed);
-        if (c > 0) return c;
-    }
-    int n = 0;
-    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess) return 0;
-    if (dev < 64) cache[dev].store(n, std::memory_order_relaxed);
-    return n;
 }
 
 // Units per (group, head) of a launch that runs as units of 32 rows (short
