@@ -1,6 +1,6 @@
-"""ctypes binding of the C ABI in ``include/h3attn.h``.
+"""ctypes binding of the C ABI in ``include/h3attn.h`` and ``include/h3block.h``.
 
-The structures below mirror the header's argument structs field for field. Loading fails loudly (``RuntimeError``) when the library has
+The structures below mirror the headers' argument structs field for field. Loading fails loudly (``RuntimeError``) when the library has
 not been built: there is no other implementation behind these entry points.
 """
 
@@ -280,7 +280,124 @@ class ProjArgs(ctypes.Structure):
     ]
 
 
-# Every function the header declares, with its ctypes signature.
+# Activations of h3a_linear (H3A_ACT_*).
+ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2, "gelu_tanh": 3, "relu": 4}
+
+H3A_BLOCK_Q = 256  # query rows of a block list
+H3A_BLOCK_K = 64   # keys of a listed block
+H3A_SPARSE_MAX_BLOCKS = 7168
+
+
+class LinearArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("x", ctypes.c_void_p),
+        ("weight", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("bias_dtype", ctypes.c_int32),
+        ("residual", ctypes.c_void_p),
+        ("gate", ctypes.c_void_p),
+        ("gate_dtype", ctypes.c_int32),
+        ("gate_stride", ctypes.c_int64),
+        ("table_rows", ctypes.c_int64),
+        ("index", ctypes.c_void_p),
+        ("index_dtype", ctypes.c_int32),
+        ("n_index", ctypes.c_int64),
+        ("y", ctypes.c_void_p),
+        ("m", ctypes.c_int64),
+        ("k", ctypes.c_int64),
+        ("n", ctypes.c_int64),
+        ("x_stride", ctypes.c_int64),
+        ("weight_stride", ctypes.c_int64),
+        ("residual_stride", ctypes.c_int64),
+        ("y_stride", ctypes.c_int64),
+        ("activation", ctypes.c_int32),
+        ("gated", ctypes.c_int32),
+    ]
+
+
+class RmsnormResidualGateRmsnormModulateArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("residual", ctypes.c_void_p),
+        ("branch", ctypes.c_void_p),
+        ("hidden_out", ctypes.c_void_p),
+        ("normed_out", ctypes.c_void_p),
+        ("branch_weight", ctypes.c_void_p),
+        ("weight", ctypes.c_void_p),
+        ("w_dtype", ctypes.c_int32),
+        ("gate", ctypes.c_void_p),
+        ("scale", ctypes.c_void_p),
+        ("shift", ctypes.c_void_p),
+        ("table_dtype", ctypes.c_int32),
+        ("gate_stride", ctypes.c_int64),
+        ("scale_stride", ctypes.c_int64),
+        ("shift_stride", ctypes.c_int64),
+        ("table_rows", ctypes.c_int64),
+        ("index", ctypes.c_void_p),
+        ("index_dtype", ctypes.c_int32),
+        ("n_index", ctypes.c_int64),
+        ("rows", ctypes.c_int64),
+        ("cols", ctypes.c_int64),
+        ("residual_stride", ctypes.c_int64),
+        ("branch_stride", ctypes.c_int64),
+        ("hidden_stride", ctypes.c_int64),
+        ("normed_stride", ctypes.c_int64),
+        ("residual_scale", ctypes.c_float),
+        ("eps", ctypes.c_float),
+    ]
+
+
+class BlockSelectArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("always", ctypes.c_void_p),
+        ("index", ctypes.c_void_p),
+        ("batch", ctypes.c_int64),
+        ("heads", ctypes.c_int64),
+        ("seqlen_q", ctypes.c_int64),
+        ("seqlen_k", ctypes.c_int64),
+        ("head_dim", ctypes.c_int64),
+        ("q_stride", _I64x3),
+        ("k_stride", _I64x3),
+        ("topk", ctypes.c_int64),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+    ]
+
+
+class AttnSparseArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("o", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("batch", ctypes.c_int64),
+        ("heads", ctypes.c_int64),
+        ("seqlen_q", ctypes.c_int64),
+        ("seqlen_k", ctypes.c_int64),
+        ("head_dim", ctypes.c_int64),
+        ("q_stride", _I64x3),
+        ("k_stride", _I64x3),
+        ("v_stride", _I64x3),
+        ("o_stride", _I64x3),
+        ("lse_stride", _I64x2),
+        ("softmax_scale", ctypes.c_float),
+        ("block_index", ctypes.c_void_p),
+        ("index_stride", _I64x3),
+        ("block_count", ctypes.c_void_p),
+        ("count_stride", _I64x3),
+        ("max_blocks", ctypes.c_int64),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+    ]
+
+
+# Every function the headers declare, with its ctypes signature.
 SIGNATURES = {
     "h3a_attn_fwd": (ctypes.c_int, [ctypes.POINTER(AttnArgs), ctypes.c_void_p]),
     "h3a_attn_fwd_workspace_size": (ctypes.c_int64, [ctypes.POINTER(AttnArgs)]),
@@ -297,6 +414,15 @@ SIGNATURES = {
     "h3a_swiglu": (ctypes.c_int, [ctypes.POINTER(SwigluArgs), ctypes.c_void_p]),
     "h3a_attn_merge": (ctypes.c_int, [ctypes.POINTER(AttnMergeArgs), ctypes.c_void_p]),
     "h3a_proj_gemm": (ctypes.c_int, [ctypes.POINTER(ProjArgs), ctypes.c_void_p]),
+    "h3a_linear": (ctypes.c_int, [ctypes.POINTER(LinearArgs), ctypes.c_void_p]),
+    "h3a_rmsnorm_residual_gate_rmsnorm_modulate": (
+        ctypes.c_int,
+        [ctypes.POINTER(RmsnormResidualGateRmsnormModulateArgs), ctypes.c_void_p],
+    ),
+    "h3a_block_select": (ctypes.c_int, [ctypes.POINTER(BlockSelectArgs), ctypes.c_void_p]),
+    "h3a_block_select_workspace_size": (ctypes.c_int64, [ctypes.POINTER(BlockSelectArgs)]),
+    "h3a_attn_sparse": (ctypes.c_int, [ctypes.POINTER(AttnSparseArgs), ctypes.c_void_p]),
+    "h3a_attn_sparse_workspace_size": (ctypes.c_int64, [ctypes.POINTER(AttnSparseArgs)]),
     "h3a_clock_sample": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
     "h3a_last_error": (ctypes.c_char_p, []),
     "h3a_abi_version": (ctypes.c_int, []),
@@ -426,6 +552,14 @@ residual_gate_rmsnorm_modulate = Launch("h3a_residual_gate_rmsnorm_modulate", Re
 swiglu = Launch("h3a_swiglu", SwigluArgs)
 attn_merge = Launch("h3a_attn_merge", AttnMergeArgs)
 proj_gemm = Launch("h3a_proj_gemm", ProjArgs)
+linear = Launch("h3a_linear", LinearArgs)
+rmsnorm_residual_gate_rmsnorm_modulate = Launch(
+    "h3a_rmsnorm_residual_gate_rmsnorm_modulate", RmsnormResidualGateRmsnormModulateArgs
+)
+block_select = Launch("h3a_block_select", BlockSelectArgs)
+block_select_workspace_size = Launch("h3a_block_select_workspace_size", BlockSelectArgs, ctypes.c_int64, on_stream=False)
+attn_sparse = Launch("h3a_attn_sparse", AttnSparseArgs)
+attn_sparse_workspace_size = Launch("h3a_attn_sparse_workspace_size", AttnSparseArgs, ctypes.c_int64, on_stream=False)
 
 
 def provenance() -> dict:

@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include "h3attn.h"
+#include "h3block.h"
 
 namespace h3a {
 
@@ -284,6 +285,75 @@ struct ProjGemmParams {
 int proj_gemm_tile();        // the largest tile's extent in features and in tokens
 int proj_gemm_k_multiple();  // k must be a multiple of this
 hipError_t launch_proj_gemm(ProjGemmParams p, int cus, hipStream_t stream);
+
+// Matrix product with bias, activation, gate and residual. Byte strides.
+struct LinearParams {
+    const void* x;         // bf16 (m, k)
+    const void* w;         // bf16 (n or, gated, 2 n, k)
+    const void* bias;      // bf16 or fp32, as many as w has rows, or NULL
+    const void* residual;  // bf16 (m, n) or NULL
+    const void* gate;      // bf16 or fp32 (table_rows, n) or NULL
+    const void* index;     // int32 or int64 (gate != NULL)
+    void* y;               // bf16 (m, n)
+    int64_t x_rs, w_rs, y_rs, res_rs, gate_rs;
+    int64_t table_rows, n_index;
+    int32_t m, k, n;       // k and n multiples of 8
+    int32_t act, gated, bias_f32, gate_f32, index_i64;
+    int32_t m_tiles, n_tiles, group_m;  // set by the launcher
+};
+int linear_max_tile();  // rows of an operand that one buffer resource spans at most
+hipError_t launch_linear(LinearParams p, int cus, hipStream_t stream);
+
+// Norm of a branch, gate, scaled residual, norm and modulation. Strides in elements.
+struct SandwichParams {
+    const void* branch;
+    const void* residual;
+    void* hidden;
+    void* out;  // NULL: the pass ends at hidden
+    const void* branch_weight;
+    const void* weight;
+    const void* gate;  // NULL: 1
+    const void* scale;
+    const void* shift;
+    const void* index;  // NULL: no table is read
+    int64_t branch_stride, residual_stride, hidden_stride, out_stride;
+    int64_t gate_stride, scale_stride, shift_stride;
+    int64_t rows, n_index, table_rows;
+    int32_t cols;
+    int32_t w_f32, table_f32, index_i64;
+    float residual_scale, eps;
+};
+hipError_t launch_sandwich(const SandwichParams& p, bool vec, hipStream_t stream);
+
+// Key-block selection. Strides: batch and head in elements, rows in bytes.
+constexpr int kSelectBlockQ = H3A_BLOCK_Q, kSelectBlockK = H3A_BLOCK_K;
+struct SelectParams {
+    const void* q;
+    const void* k;
+    int64_t q_sb, q_sh, q_rs, k_sb, k_sh, k_rs;
+    const uint8_t* always;  // (nk,) or NULL
+    int32_t* index;         // (batch, heads, nq, topk)
+    float* qm;              // workspace: means (batch, heads, nq, 128) and (.., nk, 128), scores (.., nq, nk)
+    float* km;
+    float* score;
+    int32_t batch, heads, seqlen_q, seqlen_k, nq, nk, topk;
+};
+int select_max_blocks();  // most key blocks of a row
+hipError_t launch_block_select(const SelectParams& p, hipStream_t stream);
+
+// Attention over lists of key blocks: a dense launch description (its ws_o /
+// ws_lse hold pieces x tiles partial results, in fp32) and the lists.
+struct SparseParams : AttnParams {
+    const int32_t* list;   // max_blocks entries per (batch, head, query tile)
+    const int32_t* count;  // entries used, or NULL: all
+    int64_t list_sb, list_sh, list_sq, count_sb, count_sh, count_sq;  // elements
+    int32_t max_blocks;
+    int32_t pieces;        // parts of a tile's list, 1: none
+};
+constexpr int kListMax = H3A_SPARSE_MAX_BLOCKS;
+// Chooses the form: units for few rows (n_units), or tiles, in how many pieces.
+void plan_attn_sparse(SparseParams& p, int cus);
+hipError_t launch_attn_sparse(const SparseParams& p, hipStream_t stream);
 
 // Clock sample (clock.hip): H3A_CLOCK_RECORDS records of 4 uint64 at out.
 hipError_t launch_clock_sample(uint64_t* out, hipStream_t stream);

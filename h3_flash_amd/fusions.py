@@ -8,6 +8,9 @@ wrappers (src/h3_flash/runtime/kernels/fusions.py):
 * :func:`fused_swiglu` (fusions.py:251-265)
 * :func:`fused_qknorm_rope` (fusions.py:268-293), from :mod:`h3_flash_amd.prologue`
 
+and, for blocks that also normalise what a branch returns,
+:func:`fused_rmsnorm_residual_gate_rmsnorm_modulate`, which the reference lacks.
+
 Activations are bf16 (the dtype the H3 block runs in); weights and
 modulation tables may be bf16 or fp32, table indices int32 or int64. Table
 indices outside the table are clamped to it (the reference reads out of
@@ -25,6 +28,7 @@ __all__ = [
     "fused_qknorm_rope",
     "fused_residual_gate_rmsnorm_modulate",
     "fused_rmsnorm_modulate",
+    "fused_rmsnorm_residual_gate_rmsnorm_modulate",
     "fused_swiglu",
 ]
 
@@ -127,6 +131,59 @@ def fused_residual_gate_rmsnorm_modulate(residual, branch, gate, weight, scale, 
         residual_flat.stride(0), branch_flat.stride(0), hidden.stride(0), normed.stride(0), float(eps),
     )
     return hidden.view(residual.shape), normed.view(residual.shape)
+
+
+def fused_rmsnorm_residual_gate_rmsnorm_modulate(
+    residual, branch, branch_weight, gate, weight, scale, shift, index, eps, *, residual_scale=1.0
+):
+    """``hidden = residual_scale * residual + gate[t] * RMSNorm(branch) *
+    branch_weight``, then ``RMSNorm(hidden) * weight * (1 + scale[t]) +
+    shift[t]``; returns ``(hidden, normed)``.
+
+    ``gate=None`` leaves the gate out. ``weight=None`` (with ``scale`` and
+    ``shift`` None) ends at the hidden state, as after a model's last block, and
+    returns ``(hidden, None)``; ``index`` may be None when no table is given."""
+
+    columns = residual.shape[-1]
+    if branch.shape != residual.shape:
+        raise ValueError(f"residual {tuple(residual.shape)} and branch {tuple(branch.shape)} differ")
+    if (weight is None) != (scale is None) or (weight is None) != (shift is None):
+        raise ValueError("weight, scale and shift go together: give all three or none")
+    device = residual.device
+    residual_flat = _rows(residual, "residual", columns)
+    branch_flat = _rows(branch, "branch", columns)
+    if branch.device != device:
+        raise ValueError(f"residual and branch must be on one device, got {device} and {branch.device}")
+    weights = [_vector(branch_weight, columns, device, "branch_weight")]
+    if weight is not None:
+        weights.append(_vector(weight, columns, device, "weight"))
+        if weights[0].dtype != weights[1].dtype:  # one dtype for both
+            weights = [w.float() for w in weights]
+    given = [t for t in (gate, scale, shift) if t is not None]
+    tables = _tables(given, columns, device) if given else []
+    if tables and index is None:
+        raise ValueError("gate, scale and shift need an index")
+    spread = iter(tables)
+    gate_args, scale_args, shift_args = (
+        (0, 0) if t is None else (lambda m: (m.data_ptr(), m.stride(0)))(next(spread)) for t in (gate, scale, shift)
+    )
+    index_args = (0, _ext.H3A_DTYPE_I64, 0)
+    if tables:
+        index = _index(index, device)
+        index_args = _index_args(index)
+    rows = residual_flat.shape[0]
+    hidden = residual_flat.new_empty((rows, columns))
+    normed = residual_flat.new_empty((rows, columns)) if weight is not None else None
+    if columns:
+        _ext.rmsnorm_residual_gate_rmsnorm_modulate.run(
+            device, _ext.ABI_VERSION, residual_flat.data_ptr(), branch_flat.data_ptr(), hidden.data_ptr(),
+            0 if normed is None else normed.data_ptr(), weights[0].data_ptr(), 0 if weight is None else weights[1].data_ptr(),
+            _dtype(weights[0]), gate_args[0], scale_args[0], shift_args[0],
+            _dtype(tables[0]) if tables else _ext.H3A_DTYPE_BF16, gate_args[1], scale_args[1], shift_args[1],
+            min((t.shape[0] for t in tables), default=0), *index_args, rows, columns, residual_flat.stride(0),
+            branch_flat.stride(0), hidden.stride(0), columns, float(residual_scale), float(eps),
+        )
+    return hidden.view(residual.shape), None if normed is None else normed.view(residual.shape)
 
 
 def fused_swiglu(x):
