@@ -251,7 +251,7 @@ const Shape* pick_shape(const LinearParams& p, int cus) {
 // waves' partial sums meet in LDS, in wave order.
 template <int NB, bool kGated>
 __global__ __launch_bounds__(1024) void linear_rows_kernel(LinearParams p) {
-    constexpr int kS = kGated ? 2 : 1, kU = NB + kS == 2 ? 4 : 2;
+    constexpr int kS = kGated ? 2 : 1, kU = NB + kS == 2 ? 8 : 4;
     extern __shared__ f32x4 part[];  // [wave][kS * NB][64]
     const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, l15 = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = (int)blockDim.x >> 6;
@@ -279,7 +279,7 @@ __global__ __launch_bounds__(1024) void linear_rows_kernel(LinearParams p) {
                 in[u][h] = at < bytes;
                 const int o = in[u][h] ? at : bytes - 16;
 #pragma unroll
-                for (int s = 0; s < kS; ++s) w[u][h][s] = __builtin_nontemporal_load((const i32x4*)(wr[s] + o));
+                for (int s = 0; s < kS; ++s) w[u][h][s] = *(const i32x4*)(wr[s] + o);
 #pragma unroll
                 for (int b = 0; b < NB; ++b) x[u][h][b] = *(const i32x4*)(xr[b] + o);
             }
