@@ -313,6 +313,8 @@ class LinearArgs(ctypes.Structure):
         ("y_stride", ctypes.c_int64),
         ("activation", ctypes.c_int32),
         ("gated", ctypes.c_int32),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
     ]
 
 
@@ -415,6 +417,7 @@ SIGNATURES = {
     "h3a_attn_merge": (ctypes.c_int, [ctypes.POINTER(AttnMergeArgs), ctypes.c_void_p]),
     "h3a_proj_gemm": (ctypes.c_int, [ctypes.POINTER(ProjArgs), ctypes.c_void_p]),
     "h3a_linear": (ctypes.c_int, [ctypes.POINTER(LinearArgs), ctypes.c_void_p]),
+    "h3a_linear_workspace_size": (ctypes.c_int64, [ctypes.POINTER(LinearArgs)]),
     "h3a_rmsnorm_residual_gate_rmsnorm_modulate": (
         ctypes.c_int,
         [ctypes.POINTER(RmsnormResidualGateRmsnormModulateArgs), ctypes.c_void_p],
@@ -553,6 +556,7 @@ swiglu = Launch("h3a_swiglu", SwigluArgs)
 attn_merge = Launch("h3a_attn_merge", AttnMergeArgs)
 proj_gemm = Launch("h3a_proj_gemm", ProjArgs)
 linear = Launch("h3a_linear", LinearArgs)
+linear_workspace_size = Launch("h3a_linear_workspace_size", LinearArgs, ctypes.c_int64, on_stream=False)
 rmsnorm_residual_gate_rmsnorm_modulate = Launch(
     "h3a_rmsnorm_residual_gate_rmsnorm_modulate", RmsnormResidualGateRmsnormModulateArgs
 )

@@ -142,12 +142,11 @@ int prepare_sparse(const h3a_attn_sparse_args* a, h3a::SparseParams& p, int64_t*
     return H3A_OK;
 }
 
-}  // namespace
-
-extern "C" {
-
-int h3a_linear(const h3a_linear_args* a, void* stream) {
-    h3a::clear_error();
+// Fills the launch description; *need: the workspace of its pieces, *empty:
+// nothing to launch.
+int prepare_linear(const h3a_linear_args* a, h3a::LinearParams& p, int64_t* need, bool* empty) {
+    *need = 0;
+    *empty = false;
     const char* fn = "h3a_linear";
     if (a == nullptr) return fail(H3A_EINVAL, "%s: args is NULL", fn);
     if (a->abi_version != H3A_ABI_VERSION)
@@ -159,7 +158,10 @@ int h3a_linear(const h3a_linear_args* a, void* stream) {
     if (a->activation < H3A_ACT_NONE || a->activation > H3A_ACT_RELU) return fail(H3A_EINVAL, "%s: unknown activation %d", fn, a->activation);
     if (a->m >= ((int64_t)1 << 31) - 256 || a->n >= ((int64_t)1 << 30) || a->k >= ((int64_t)1 << 30))
         return fail(H3A_EUNSUPPORTED, "%s: extents too large", fn);
-    if (a->m == 0) return H3A_OK;
+    if (a->m == 0) {
+        *empty = true;
+        return H3A_OK;
+    }
     const void* ptrs[3] = {a->x, a->weight, a->y};
     for (const void* q : ptrs)
         if (!q || !aligned16(q)) return fail(H3A_EINVAL, "%s: x, weight and y must be 16-byte aligned device pointers", fn);
@@ -168,7 +170,6 @@ int h3a_linear(const h3a_linear_args* a, void* stream) {
     const int64_t rows = h3a::linear_max_tile();
     if (a->x_stride > (kMaxSpan - 1) / (2 * rows) || a->weight_stride > (kMaxSpan - 1) / (2 * rows))
         return fail(H3A_EUNSUPPORTED, "%s: %lld rows of x and of weight must span less than 2^31 bytes", fn, (long long)rows);
-    h3a::LinearParams p{};
     if (a->bias != nullptr) {
         if (!bf16_or_f32(a->bias_dtype)) return fail(H3A_EINVAL, "%s: unknown bias dtype %d", fn, a->bias_dtype);
         if (!aligned16(a->bias)) return fail(H3A_EINVAL, "%s: bias must be 16-byte aligned", fn);
@@ -202,6 +203,40 @@ int h3a_linear(const h3a_linear_args* a, void* stream) {
     p.x_rs = a->x_stride * 2; p.w_rs = a->weight_stride * 2; p.y_rs = a->y_stride * 2;
     p.m = (int32_t)a->m; p.k = (int32_t)a->k; p.n = (int32_t)a->n;
     p.act = a->activation; p.gated = a->gated != 0;
+    h3a::plan_linear(p, h3a::device_cus(), need);
+    return H3A_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t h3a_linear_workspace_size(const h3a_linear_args* a) {
+    h3a::clear_error();
+    h3a::LinearParams p{};
+    int64_t need = 0;
+    bool empty = false;
+    const int rc = prepare_linear(a, p, &need, &empty);
+    return rc != H3A_OK ? rc : need;
+}
+
+int h3a_linear(const h3a_linear_args* a, void* stream) {
+    h3a::clear_error();
+    const char* fn = "h3a_linear";
+    h3a::LinearParams p{};
+    int64_t need = 0;
+    bool empty = false;
+    const int rc = prepare_linear(a, p, &need, &empty);
+    if (rc != H3A_OK || empty) return rc;
+    if (need > 0) {
+        if (a->workspace == nullptr && a->workspace_bytes == H3A_WORKSPACE_ASK) return H3A_NEED_WORKSPACE;
+        if (a->workspace != nullptr && ((uintptr_t)a->workspace & 255u) == 0 && a->workspace_bytes >= need) {
+            p.ws = a->workspace;
+        } else {
+            p.n_full = p.m_tiles * p.n_tiles;  // every tile whole
+            p.split = 1;
+        }
+    }
     const hipError_t e = h3a::launch_linear(p, h3a::device_cus(), (hipStream_t)stream);
     if (e != hipSuccess) return fail(H3A_ELAUNCH, "%s: launch failed: %s", fn, hipGetErrorString(e));
     return H3A_OK;

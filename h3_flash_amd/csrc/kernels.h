@@ -299,10 +299,16 @@ struct LinearParams {
     int64_t table_rows, n_index;
     int32_t m, k, n;       // k and n multiples of 8
     int32_t act, gated, bias_f32, gate_f32, index_i64;
-    int32_t m_tiles, n_tiles, group_m;  // set by the launcher
+    // Set by plan_linear: the tile shape (-1: the form for few tokens), its tiles
+    // over tokens and features, the token tiles of a group of their order, and
+    // of the tiles past n_full the pieces along K, whose sums go to ws.
+    int32_t shape, m_tiles, n_tiles, group_m, n_full, split;
+    void* ws;
 };
 int linear_max_tile();  // rows of an operand that one buffer resource spans at most
-hipError_t launch_linear(LinearParams p, int cus, hipStream_t stream);
+// Chooses the form; *workspace: the bytes that its pieces take (0: none).
+void plan_linear(LinearParams& p, int cus, int64_t* workspace);
+hipError_t launch_linear(const LinearParams& p, int cus, hipStream_t stream);
 
 // Norm of a branch, gate, scaled residual, norm and modulation. Strides in elements.
 struct SandwichParams {

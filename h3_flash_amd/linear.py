@@ -97,10 +97,17 @@ def fused_linear(
         if m and (y.stride(1) != 1 or y.stride(0) % 8 or y.stride(0) < n or y.data_ptr() % 16):
             raise ValueError("out must have contiguous, 16-byte aligned rows")
     if m:
-        _ext.linear.run(
-            device, _ext.ABI_VERSION, flat.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(),
+        args = (
+            _ext.ABI_VERSION, flat.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(),
             _ext.H3A_DTYPE_BF16 if bias is None else _dtype(bias), 0 if residual is None else residual.data_ptr(), *gate_args,
             y.data_ptr(), m, k, n, flat.stride(0), weight.stride(0), 0 if residual is None else residual.stride(0), y.stride(0),
             _ext.ACTIVATIONS[activation], int(gated),
         )
+        rc = _ext.linear(device, *args, 0, _ext.H3A_WORKSPACE_ASK)
+        if rc == _ext.H3A_NEED_WORKSPACE:
+            need = _ext.linear_workspace_size(device, *args, 0, 0)
+            workspace = torch.empty(need, dtype=torch.uint8, device=device)
+            rc = _ext.linear(device, *args, workspace.data_ptr(), need)
+        if rc != _ext.H3A_OK:
+            _ext.check(_ext.load_library(), rc)
     return out

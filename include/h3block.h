@@ -29,6 +29,11 @@ extern "C" {
  * rows are 16-byte aligned (strides multiples of 8 elements; fp32 gate rows of
  * 4); 256 rows of x and of weight span less than 2^31 bytes. y may be the
  * residual, and must not overlap any other operand.
+ * A launch whose last round of tiles would leave CUs idle cuts those tiles into
+ * pieces along k, whose sums (fp32) take a workspace of
+ * h3a_linear_workspace_size bytes, 256-byte aligned; without one every tile runs
+ * whole. workspace NULL with workspace_bytes H3A_WORKSPACE_ASK: the call
+ * launches, or returns H3A_NEED_WORKSPACE without launching where it takes one.
  */
 #define H3A_ACT_NONE 0
 #define H3A_ACT_SILU 1
@@ -60,8 +65,11 @@ typedef struct h3a_linear_args {
     int64_t y_stride;
     int32_t activation;
     int32_t gated;
+    void *workspace;
+    int64_t workspace_bytes;
 } h3a_linear_args;
 
+H3A_API int64_t h3a_linear_workspace_size(const h3a_linear_args *args);
 H3A_API int h3a_linear(const h3a_linear_args *args, void *stream);
 
 /*

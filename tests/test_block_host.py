@@ -45,6 +45,7 @@ def test_every_declared_function_is_exported_and_bound(lib):
         "h3a_block_select",
         "h3a_block_select_workspace_size",
         "h3a_linear",
+        "h3a_linear_workspace_size",
         "h3a_rmsnorm_residual_gate_rmsnorm_modulate",
     ]
     for name in names:
