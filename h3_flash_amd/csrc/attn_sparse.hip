@@ -10,6 +10,8 @@
 // so the tile's pipeline runs as in the dense forward with the list in place of
 // the key range. Every workgroup first packs its list into LDS, without the
 // entries that name nothing: no content of a list can address outside K or V.
+#include <math.h>
+
 #include "attn_tile.h"
 #include "common.h"
 #include "kernels.h"
@@ -93,19 +95,39 @@ __global__ __launch_bounds__(kThreads, 2) void attn_sparse_short_kernel(SparsePa
 
 }  // namespace
 
+// Expected time (us) of `jobs` tiles or pieces over kt listed blocks each: rounds
+// over the CUs of a fixed part and the blocks, slower the more CUs are busy.
+static double round_us(int64_t jobs, double kt, int cus) {
+    const double busy = jobs < cus ? (double)jobs / (double)cus : 1.0;
+    return (double)((jobs + cus - 1) / cus) * (9.7 + kt * (1.0 + 0.6 * busy));
+}
+
+// Units of 32 rows, whole tiles, or (for less than a round of tiles) tiles in
+// pieces, by the expected time. A round of units: 5 us and 1.5 per 256 keys, a
+// tenth more in practice; pieces: the merge, 3 us and 0.055 a piece (its fp32
+// partial rows written and read). On 17 sizes of 1 to 24,960 rows, 4 to 40 heads
+// and 3 to 150 blocks, each run as units, whole and in 2 to 8 pieces, this picks
+// the fastest or one within 6% of it (us, units / whole / best in pieces: 4 heads
+// of 4,095 x 16 blocks 26 / 28 / 31; 20 of 2,048 x 8 46 / 22 / 41; 20 of 512 x 32
+// 35 / 45 / 29; 8 of 512 x 16 12 / 26 / 20; 5 of 256 x 150 55 / 172 / 38).
 void plan_attn_sparse(SparseParams& p, int cus) {
     const int64_t tiles = (int64_t)p.n_qtiles * p.heads * p.n_groups;
     if (cus <= 0 || p.max_blocks == 0) return;
-    // Few rows: units, while they all run at once over short lists.
-    const int64_t units = (int64_t)((p.seqlen_q + kUnitRows - 1) / kUnitRows) * p.heads * p.n_groups;
-    if (units <= cus && p.max_blocks <= 48) {
-        p.n_units = (p.seqlen_q + kUnitRows - 1) / kUnitRows;
-        return;
+    const double n = (double)p.max_blocks;
+    const int32_t per = (p.seqlen_q + kUnitRows - 1) / kUnitRows;
+    const int64_t units = (int64_t)per * p.heads * p.n_groups;
+    const double units_us = 1.15 * (double)((units + cus - 1) / cus) * (4.8 + 1.5 * ceil(n * kBN / 256.0));
+    double best = round_us(tiles, n, cus);
+    for (int c = 2; c <= 8 && c <= p.max_blocks && tiles < cus; ++c) {
+        const double us = round_us(tiles * c, n / c, cus) + 3.0 + 0.055 * (double)(tiles * c);
+        if (us < best) {
+            best = us;
+            p.pieces = c;
+        }
     }
-    if (tiles < cus) {
-        const SplitPlan plan = plan_attn_split(tiles, p.max_blocks, cus, INT64_MAX);
-        if (plan.split_n > 1) p.pieces = plan.split_n;
-    }
+    if (units_us >= best) return;
+    p.pieces = 1;
+    p.n_units = per;
 }
 
 hipError_t launch_attn_sparse(const SparseParams& p, hipStream_t stream) {
