@@ -74,34 +74,45 @@ __global__ __launch_bounds__(256) void block_mean_kernel(SelectParams p) {
 
 // ---------------------------------------------------------------- scores
 
-// One wave per 16 query blocks x 16 key blocks. A lane holds, of its row of each
-// operand, columns 32 (l >> 4) .. +32: MFMA step s multiplies column 32 g + s of
-// every lane group g. The result: column l & 15, rows (l >> 4) + 4 i.
+// One wave per 16 query blocks x 32 key blocks: two chains of products. Lane l
+// holds, of row l & 15 of each operand, columns 16 i + 4 g .. +4 (g = l >> 4) for
+// i = 0 .. 7, so that the four lanes of a row load 64 bytes side by side; MFMA
+// step (i, e) multiplies column 16 i + 4 g + e of every lane group. The result:
+// column l & 15, rows g + 4 i. (With 32 columns of a lane in one piece, 64 lines
+// a load, 780 x 195 blocks at 5 heads took 13.5 us.)
+constexpr int kKT = 2;
+
 __global__ __launch_bounds__(256) void block_score_kernel(SelectParams p) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t bh = blockIdx.y;
-    const int ktiles = (p.nk + 15) / 16;
-    const int qt = (int)(blockIdx.x / ((ktiles + 3) / 4)), kt = (int)(blockIdx.x % ((ktiles + 3) / 4)) * 4 + wave;
-    if (kt >= ktiles) return;
+    const int groups = (p.nk + 16 * kKT * 4 - 1) / (16 * kKT * 4);  // of a workgroup's key blocks
+    const int qt = (int)(blockIdx.x / groups), k0 = ((int)(blockIdx.x % groups) * 4 + wave) * 16 * kKT;
+    if (k0 >= p.nk) return;
     const int l15 = lane & 15, g = lane >> 4;
-    const float* const qr = p.qm + (bh * p.nq + min(qt * 16 + l15, p.nq - 1)) * kD + 32 * g;
-    const float* const kr = p.km + (bh * p.nk + min(kt * 16 + l15, p.nk - 1)) * kD + 32 * g;
-    f32x4 a[8], b[8];
+    const float* const qr = p.qm + (bh * p.nq + min(qt * 16 + l15, p.nq - 1)) * kD + 4 * g;
+    const float* kr[kKT];
+#pragma unroll
+    for (int t = 0; t < kKT; ++t) kr[t] = p.km + (bh * p.nk + min(k0 + 16 * t + l15, p.nk - 1)) * kD + 4 * g;
+    f32x4 a[8], b[kKT][8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        a[i] = *(const f32x4*)(qr + 4 * i);
-        b[i] = *(const f32x4*)(kr + 4 * i);
+        a[i] = *(const f32x4*)(qr + 16 * i);
+#pragma unroll
+        for (int t = 0; t < kKT; ++t) b[t][i] = *(const f32x4*)(kr[t] + 16 * i);
     }
-    f64x4 acc{};
+    f64x4 acc[kKT] = {};
 #pragma unroll
     for (int s = 0; s < 32; ++s)
-        acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)a[s >> 2][s & 3], (double)b[s >> 2][s & 3], acc, 0, 0, 0);
-    const int col = kt * 16 + l15;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int row = qt * 16 + g + 4 * i;
-        if (row < p.nq && col < p.nk) p.score[(bh * p.nq + row) * p.nk + col] = (float)acc[i];
-    }
+        for (int t = 0; t < kKT; ++t)
+            acc[t] = __builtin_amdgcn_mfma_f64_16x16x4f64((double)a[s >> 2][s & 3], (double)b[t][s >> 2][s & 3], acc[t], 0, 0, 0);
+#pragma unroll
+    for (int t = 0; t < kKT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = qt * 16 + g + 4 * i, col = k0 + 16 * t + l15;
+            if (row < p.nq && col < p.nk) p.score[(bh * p.nq + row) * p.nk + col] = (float)acc[t][i];
+        }
 }
 
 // ---------------------------------------------------------------- choice
@@ -124,11 +135,27 @@ __global__ __launch_bounds__(64 * kWaves) void block_choose_kernel(SelectParams 
     const int64_t row = blockIdx.x;
     const float* const score = p.score + row * p.nk;
     uint32_t key[kR];
+    // Loads in groups, past the row from its last block: behind a branch each
+    // would wait for the one before it.
+    constexpr int kG = kR < 16 ? kR : 16;
 #pragma unroll
-    for (int r = 0; r < kR; ++r) {
-        const int j = (r * kWaves + wave) * 64 + lane;
-        key[r] = 0;  // past the row: below every score
-        if (j < p.nk) key[r] = p.always != nullptr && p.always[j] != 0 ? 0xffffffffu : order_key(score[j]);
+    for (int r0 = 0; r0 < kR; r0 += kG) {
+        float s[kG];
+        uint32_t marked[kG];
+#pragma unroll
+        for (int r = 0; r < kG; ++r) s[r] = score[min(((r0 + r) * kWaves + wave) * 64 + lane, p.nk - 1)];
+        if (p.always != nullptr) {
+#pragma unroll
+            for (int r = 0; r < kG; ++r) marked[r] = p.always[min(((r0 + r) * kWaves + wave) * 64 + lane, p.nk - 1)];
+        } else {
+#pragma unroll
+            for (int r = 0; r < kG; ++r) marked[r] = 0;
+        }
+#pragma unroll
+        for (int r = 0; r < kG; ++r) {
+            const uint32_t k = marked[r] != 0 ? 0xffffffffu : order_key(s[r]);
+            key[r0 + r] = ((r0 + r) * kWaves + wave) * 64 + lane < p.nk ? k : 0;  // past the row: below every score
+        }
     }
     // Number of the row's keys at or above x.
     int turn = 0;
@@ -204,7 +231,7 @@ int select_max_blocks() { return 32 * 64 * 16; }
 hipError_t launch_block_select(const SelectParams& p, hipStream_t stream) {
     const int64_t bh = (int64_t)p.batch * p.heads;
     hipLaunchKernelGGL(block_mean_kernel, dim3((unsigned)(bh * (p.nq + p.nk))), dim3(256), 0, stream, p);
-    const int64_t qtiles = (p.nq + 15) / 16, kgroups = ((p.nk + 15) / 16 + 3) / 4;
+    const int64_t qtiles = (p.nq + 15) / 16, kgroups = (p.nk + 16 * kKT * 4 - 1) / (16 * kKT * 4);
     hipLaunchKernelGGL(block_score_kernel, dim3((unsigned)(qtiles * kgroups), (unsigned)bh), dim3(256), 0, stream, p);
     const dim3 rows((unsigned)(bh * p.nq));
     auto choose = [&](auto kernel, int threads) { hipLaunchKernelGGL(kernel, rows, dim3(threads), 0, stream, p); };
