@@ -19,24 +19,22 @@
 namespace h3a {
 namespace {
 
-// One wave per row, four rows per workgroup, which share the two weight rows
-// through LDS. Vectors 0 .. NV-2 of a lane lie inside the row (NV = ceil(C /
-// 512)); the last one, where it does not, is loaded from the row's last vector
-// and dropped. Every load goes out before the first sum: branch, residual and
-// gate, then scale and shift, whose latency the first sum covers.
-constexpr int kRowVecMax = 11;
-
-template <int NV, bool kNorm, bool kWF32>
-__global__ __launch_bounds__(kThreads) void sandwich_row_kernel(SandwichParams p) {
-    const int lane = threadIdx.x & 63;
+// W waves per row, 4 / W rows per workgroup, which share the two weight rows
+// through LDS (bf16 tables). Vectors 0 .. NV-2 of a lane lie inside the row (NV =
+// ceil(C / (512 W))); the last one, where it does not, is loaded from the row's
+// last vector and dropped. Branch, residual and gate are all in flight before the
+// first sum, scale and shift before the second.
+template <int W, int NV, bool kNorm, bool kWF32>
+__global__ __launch_bounds__(kThreads, 2) void sandwich_row_kernel(SandwichParams p) {
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int64_t row_id = (int64_t)blockIdx.x * kWaves + wave;  // uniform
+    const int lane = (threadIdx.x & 63) + 64 * (wave % W);  // of the row's W waves
+    const int64_t row_id = (int64_t)blockIdx.x * (kWaves / W) + wave / W;  // uniform
     const bool live = row_id < p.rows;
     const int64_t row = live ? row_id : p.rows - 1;  // a wave past the rows loads the last one, stores nothing
     const int C = p.cols;
     uint32_t off[NV];  // byte offset of vector k in a bf16 row
 #pragma unroll
-    for (int k = 0; k < NV; ++k) off[k] = (uint32_t)(lane + 64 * k) * 16u;
+    for (int k = 0; k < NV; ++k) off[k] = (uint32_t)(lane + 64 * W * k) * 16u;
     const bool last = (int)(off[NV - 1] / 2) < C;
     if (!last) off[NV - 1] = (uint32_t)(C - 8) * 2u;
 
@@ -49,7 +47,7 @@ __global__ __launch_bounds__(kThreads) void sandwich_row_kernel(SandwichParams p
     for (int k = 0; k < NV; ++k) rres[k] = __builtin_nontemporal_load((const i32x4*)(rr + off[k]));
     // The weight rows: vector i (columns 8i .. 8i+7, the last clamped into the
     // row) of row j at wl[(j * kWv + i) * kWl].
-    constexpr int kWv = NV * 64, kWl = kWF32 ? 2 : 1, kWr = kNorm ? 2 : 1;
+    constexpr int kWv = NV * 64 * W, kWl = kWF32 ? 2 : 1, kWr = kNorm ? 2 : 1;
     __shared__ i32x4 wl[kWr * kWv * kWl];
 #pragma unroll
     for (int j = 0; j < kWr; ++j) {
@@ -64,8 +62,8 @@ __global__ __launch_bounds__(kThreads) void sandwich_row_kernel(SandwichParams p
     }
     auto weight = [&](int j, int k, float* out) __attribute__((always_inline)) {
         Raw8<kWF32> w;
-        w.a = wl[(j * kWv + lane + 64 * k) * kWl];
-        if constexpr (kWF32) w.b = wl[(j * kWv + lane + 64 * k) * kWl + 1];
+        w.a = wl[(j * kWv + lane + 64 * W * k) * kWl];
+        if constexpr (kWF32) w.b = wl[(j * kWv + lane + 64 * W * k) * kWl + 1];
         unpack_raw8<kWF32>(w, out);
     };
     const int64_t t = p.index != nullptr ? table_row(p, row) : 0;
@@ -78,6 +76,29 @@ __global__ __launch_bounds__(kThreads) void sandwich_row_kernel(SandwichParams p
 #pragma unroll
         for (int k = 0; k < NV; ++k) g[k] = i32x4{0x3f803f80, 0x3f803f80, 0x3f803f80, 0x3f803f80};
     }
+    float ss = 0.f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        float b[8];
+        unpack8(rx[k], b);
+        if (k < NV - 1 || last)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ss += b[e] * b[e];
+    }
+    // Sum over the row's waves, in wave order.
+    __shared__ float red[2][kWaves];
+    auto row_sum = [&](float v, int i) __attribute__((always_inline)) {
+        if constexpr (W == 1) return v;
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) s += red[i][wave / W * W + w];
+        return s;
+    };
+    ss = wave_sum(ss);
+    if (W > 1 && (threadIdx.x & 63) == 0) red[0][wave] = ss;
+    __syncthreads();  // the weight rows are in LDS
+    const float r1 = rsqrtf(row_sum(ss, 0) / (float)C + p.eps);
+    if (W == 1 && !live) return;
     i32x4 sc[kNorm ? NV : 1], sh[kNorm ? NV : 1];
     if constexpr (kNorm) {
         const char* const scr = (const char*)p.scale + t * p.scale_stride * 2;
@@ -88,53 +109,56 @@ __global__ __launch_bounds__(kThreads) void sandwich_row_kernel(SandwichParams p
             sh[k] = *(const i32x4*)(shr + off[k]);
         }
     }
-    float ss = 0.f;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        float b[8];
-        unpack8(rx[k], b);
-        if (k < NV - 1 || last)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) ss += b[e] * b[e];
-    }
-    const float r1 = rsqrtf(wave_sum(ss) / (float)C + p.eps);
-    __syncthreads();  // the weight rows are in LDS
-    if (!live) return;
     char* const hr = (char*)p.hidden + row * p.hidden_stride * 2;
-    float h[NV][8];
-    float s2 = 0.f;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
+    auto hidden = [&](int k, float* h) __attribute__((always_inline)) {
         float b[8], r[8], gv[8], wv[8];
         unpack8(rx[k], b);
         unpack8(rres[k], r);
         unpack8(g[k], gv);
         weight(0, k, wv);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) h[k][e] = p.residual_scale * r[e] + gv[e] * (b[e] * r1 * wv[e]);
-        if (k < NV - 1 || last) {
-            __builtin_nontemporal_store(pack8(h[k]), (i32x4*)(hr + off[k]));
+        for (int e = 0; e < 8; ++e) h[e] = p.residual_scale * r[e] + gv[e] * (b[e] * r1 * wv[e]);
+    };
+    float s2 = 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s2 += h[k][e] * h[k][e];
+    for (int k = 0; k < NV; ++k) {
+        float h[8];
+        hidden(k, h);
+        if (k < NV - 1 || last) {
+            if (W == 1 || live) __builtin_nontemporal_store(pack8(h), (i32x4*)(hr + off[k]));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s2 += h[e] * h[e];
         }
     }
     if constexpr (kNorm) {
-        const float r2 = rsqrtf(wave_sum(s2) / (float)C + p.eps);
+        // h is formed again below from the raw vectors rather than held in fp32
+        // through the sum (half the registers: two waves per SIMD at NV = 11).
+#pragma unroll
+        for (int k = 0; k < NV; ++k) asm volatile("" : "+v"(rx[k]), "+v"(rres[k]), "+v"(g[k]));
+        s2 = wave_sum(s2);
+        if constexpr (W > 1) {
+            if ((threadIdx.x & 63) == 0) red[1][wave] = s2;
+            __syncthreads();
+            if (!live) return;
+        }
+        const float r2 = rsqrtf(row_sum(s2, 1) / (float)C + p.eps);
         char* const orow = (char*)p.out + row * p.out_stride * 2;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            float wv[8], scv[8], shv[8], o[8];
+            float h[8], wv[8], scv[8], shv[8], o[8];
+            hidden(k, h);
             weight(1, k, wv);
             unpack8(sc[k], scv);
             unpack8(sh[k], shv);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) o[e] = h[k][e] * r2 * wv[e] * (1.0f + scv[e]) + shv[e];
+            for (int e = 0; e < 8; ++e) o[e] = h[e] * r2 * wv[e] * (1.0f + scv[e]) + shv[e];
             if (k < NV - 1 || last) __builtin_nontemporal_store(pack8(o), (i32x4*)(orow + off[k]));
         }
     }
 }
 
-// One row per workgroup, NV vectors of 8 per thread: wider rows, fp32 tables.
+// One row per workgroup, NV vectors of 8 per thread: few rows, wide rows, fp32
+// tables.
 template <int NV, bool kTabF32, bool kWF32>
 __global__ __launch_bounds__(kThreads) void sandwich_block_kernel(SandwichParams p) {
     __shared__ float red[2][kWaves];
@@ -249,18 +273,17 @@ __global__ __launch_bounds__(kThreads) void sandwich_elem_kernel(SandwichParams 
     }
 }
 
-template <bool kNorm, bool kWF32>
+template <int W, bool kNorm, bool kWF32>
 void launch_rows(const SandwichParams& p, hipStream_t stream) {
-    const dim3 grid((unsigned)((p.rows + kWaves - 1) / kWaves)), block(kThreads);
-    switch ((p.cols + 511) / 512) {
-#define H3A_NW(n)                                                                                     \
-    case n:                                                                                           \
-        hipLaunchKernelGGL((sandwich_row_kernel<n, kNorm, kWF32>), grid, block, 0, stream, p);       \
-        break;
-        H3A_NW(1) H3A_NW(2) H3A_NW(3) H3A_NW(4) H3A_NW(5) H3A_NW(6) H3A_NW(7) H3A_NW(8)
-        H3A_NW(9) H3A_NW(10) H3A_NW(11)
-#undef H3A_NW
+    const dim3 grid((unsigned)((p.rows + kWaves / W - 1) / (kWaves / W))), block(kThreads);
+    const int nv = (p.cols + 512 * W - 1) / (512 * W);
+#define H3A_NW(n) \
+    if (nv == n) hipLaunchKernelGGL((sandwich_row_kernel<W, n, kNorm, kWF32>), grid, block, 0, stream, p);
+    if constexpr (W == 1) {
+        H3A_NW(1) H3A_NW(2) H3A_NW(3) H3A_NW(4) H3A_NW(8)
     }
+    H3A_NW(5) H3A_NW(6) H3A_NW(7)
+#undef H3A_NW
 }
 
 template <bool kTabF32, bool kWF32>
@@ -271,7 +294,7 @@ void launch_block(const SandwichParams& p, hipStream_t stream) {
     case n:                                                                                           \
         hipLaunchKernelGGL((sandwich_block_kernel<n, kTabF32, kWF32>), grid, block, 0, stream, p);   \
         break;
-        H3A_NV(1) H3A_NV(2) H3A_NV(3) H3A_NV(4)
+        H3A_NV(1) H3A_NV(2) H3A_NV(3) H3A_NV(4) H3A_NV(5) H3A_NV(6) H3A_NV(7) H3A_NV(8)
 #undef H3A_NV
     }
 }
@@ -281,12 +304,24 @@ void launch_block(const SandwichParams& p, hipStream_t stream) {
 hipError_t launch_sandwich(const SandwichParams& p, bool vec, hipStream_t stream) {
     if (p.rows == 0 || p.cols == 0) return hipSuccess;
     const bool w = p.w_f32 != 0;
-    if (vec && !p.table_f32 && p.cols <= 512 * kRowVecMax) {
+    // us by graph replays, a workgroup per row / one wave / two waves: 1,024 rows
+    // of 1,024 4.3 / 4.4 / 4.5, 2,048 of 1,024 6.4 / 5.3 / 5.6, 49,920 of 1,024 95 /
+    // 68 / 71, 2,048 of 4,096 16 / 14 / 17, 6,240 of 5,376 56 / - / 60, 12,480 of
+    // 5,376 103 / - / 105, 20,000 of 5,376 164 / - / 162, 30,000 of 6,144 276 / - /
+    // 259, 49,920 of 5,120 398 / 355 / 362. Past 4,096 columns a row takes a wave
+    // over 256 registers, past 7,168 two.
+    const int waves = !vec || p.table_f32 || p.rows <= 1024 ? 0 : p.cols <= 4096 ? 1 : p.rows > 16384 && p.cols <= 7168 ? 2 : 0;
+    if (waves == 1) {
         if (p.out != nullptr)
-            w ? launch_rows<true, true>(p, stream) : launch_rows<true, false>(p, stream);
+            w ? launch_rows<1, true, true>(p, stream) : launch_rows<1, true, false>(p, stream);
         else
-            w ? launch_rows<false, true>(p, stream) : launch_rows<false, false>(p, stream);
-    } else if (vec && p.cols <= 4 * 8 * kThreads) {
+            w ? launch_rows<1, false, true>(p, stream) : launch_rows<1, false, false>(p, stream);
+    } else if (waves == 2) {
+        if (p.out != nullptr)
+            w ? launch_rows<2, true, true>(p, stream) : launch_rows<2, true, false>(p, stream);
+        else
+            w ? launch_rows<2, false, true>(p, stream) : launch_rows<2, false, false>(p, stream);
+    } else if (vec && p.cols <= 8 * 8 * kThreads) {
         if (p.table_f32)
             w ? launch_block<true, true>(p, stream) : launch_block<true, false>(p, stream);
         else

@@ -63,6 +63,19 @@ def _run(a, eps=1e-5, **kwargs):
         (3, 8192, F32, F32, 1.0),
         (4, 8200, F32, BF16, 1.0),
         (1297, 1024, BF16, BF16, 1.0),
+        (3, 16384, BF16, F32, 1.0),
+        (2, 12296, F32, BF16, 1.0),
+        # one wave per row (past 1,024 rows, up to 4,096 columns), its last rows
+        # and vectors partial
+        (1025, 8, BF16, BF16, 1.0),
+        (1026, 1000, BF16, F32, 0.5),
+        (1027, 2056, BF16, BF16, 1.0),
+        (1029, 3600, BF16, F32, 1.0),
+        (1030, 4096, BF16, BF16, 1.0),
+        # two waves per row (past 16,384 rows)
+        (16385, 4104, BF16, BF16, 1.0),
+        (16387, 5376, BF16, F32, 0.75),
+        (16386, 7168, BF16, BF16, 1.0),
     ],
 )
 def test_parity(rows, cols, tables, weights, scale):
@@ -72,12 +85,12 @@ def test_parity(rows, cols, tables, weights, scale):
     _check(got, sandwich_reference(*a.values(), 1e-5, scale))
 
 
-@pytest.mark.parametrize("cols", [24, 1001, 5376, 6144])
-def test_without_gate_or_second_norm(cols):
-    a = _inputs(19, cols)
+@pytest.mark.parametrize("rows, cols", [(19, 24), (19, 1001), (19, 5376), (1031, 640), (16389, 4200)])
+def test_without_gate_or_second_norm(rows, cols):
+    a = _inputs(rows, cols)
     a["gate"] = None
     _check(_run(a), sandwich_reference(*a.values(), 1e-5))
-    a = _inputs(19, cols)
+    a = _inputs(rows, cols)
     a["weight"] = a["scale"] = a["shift"] = None
     _check(_run(a), sandwich_reference(*a.values(), 1e-5))
     a["gate"] = a["index"] = None
