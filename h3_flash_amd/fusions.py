@@ -40,14 +40,15 @@ def _rows(x: torch.Tensor, name: str, columns: int) -> torch.Tensor:
         raise TypeError(f"{name} must be bfloat16, got {x.dtype}")
     if not x.is_cuda:
         raise RuntimeError(f"{name} must be on a ROCm device, got {x.device}")
-    flat = x.reshape(-1, columns)
-    return flat if flat.stride(-1) == 1 else flat.contiguous()
+    flat = x if x.dim() == 2 else x.reshape(-1, columns)
+    return flat if flat.stride(1) == 1 else flat.contiguous()
 
 
 def _vector(t: torch.Tensor, columns: int, device: torch.device, name: str) -> torch.Tensor:
-    if t.shape[-1] != columns or t.numel() != columns:
-        raise ValueError(f"{name} must have {columns} elements, got shape {tuple(t.shape)}")
-    t = t.reshape(columns)
+    if t.shape != (columns,):
+        if t.shape[-1] != columns or t.numel() != columns:
+            raise ValueError(f"{name} must have {columns} elements, got shape {tuple(t.shape)}")
+        t = t.reshape(columns)
     if t.device != device:
         t = t.to(device)
     if t.dtype not in (torch.bfloat16, torch.float32):
@@ -56,21 +57,28 @@ def _vector(t: torch.Tensor, columns: int, device: torch.device, name: str) -> t
 
 
 def _tables(tables: list[torch.Tensor], columns: int, device: torch.device) -> list[torch.Tensor]:
-    out = []
+    out, dtype = [], torch.bfloat16
     for t in tables:
         if t.dim() != 2 or t.shape[1] != columns:
             raise ValueError(f"modulation tables must be (rows, {columns}), got {tuple(t.shape)}")
+        if t.dtype != torch.bfloat16:
+            dtype = torch.float32
         out.append(t if t.device == device else t.to(device))
-    dtype = torch.bfloat16 if all(t.dtype == torch.bfloat16 for t in out) else torch.float32
-    out = [t if t.dtype == dtype else t.to(dtype) for t in out]
     # _row_addressable (fusions.py:190-191): the last dimension must be
     # contiguous; broadcast rows (a row stride under the row, e.g. expand())
     # are written out, since the launch takes one row stride per table
-    return [t if t.stride(-1) == 1 and t.stride(0) >= columns else t.contiguous() for t in out]
+    for i, t in enumerate(out):
+        if t.dtype != dtype:
+            t = out[i] = t.to(dtype)
+        row, column = t.stride()
+        if column != 1 or row < columns:
+            out[i] = t.contiguous()
+    return out
 
 
 def _index(index: torch.Tensor, device: torch.device) -> torch.Tensor:
-    index = index.reshape(-1)
+    if index.dim() != 1:
+        index = index.reshape(-1)
     if index.device != device:
         index = index.to(device)
     if index.numel() == 0:
@@ -144,46 +152,48 @@ def fused_rmsnorm_residual_gate_rmsnorm_modulate(
     ``shift`` None) ends at the hidden state, as after a model's last block, and
     returns ``(hidden, None)``; ``index`` may be None when no table is given."""
 
-    columns = residual.shape[-1]
-    if branch.shape != residual.shape:
-        raise ValueError(f"residual {tuple(residual.shape)} and branch {tuple(branch.shape)} differ")
-    if (weight is None) != (scale is None) or (weight is None) != (shift is None):
+    shape = residual.shape
+    columns = shape[-1]
+    if branch.shape != shape:
+        raise ValueError(f"residual {tuple(shape)} and branch {tuple(branch.shape)} differ")
+    norm = weight is not None
+    if norm != (scale is not None) or norm != (shift is not None):
         raise ValueError("weight, scale and shift go together: give all three or none")
     device = residual.device
-    residual_flat = _rows(residual, "residual", columns)
-    branch_flat = _rows(branch, "branch", columns)
+    rows_r, rows_b = _rows(residual, "residual", columns), _rows(branch, "branch", columns)
     if branch.device != device:
         raise ValueError(f"residual and branch must be on one device, got {device} and {branch.device}")
-    weights = [_vector(branch_weight, columns, device, "branch_weight")]
-    if weight is not None:
-        weights.append(_vector(weight, columns, device, "weight"))
-        if weights[0].dtype != weights[1].dtype:  # one dtype for both
-            weights = [w.float() for w in weights]
-    given = [t for t in (gate, scale, shift) if t is not None]
-    tables = _tables(given, columns, device) if given else []
-    if tables and index is None:
-        raise ValueError("gate, scale and shift need an index")
-    spread = iter(tables)
-    gate_args, scale_args, shift_args = (
-        (0, 0) if t is None else (lambda m: (m.data_ptr(), m.stride(0)))(next(spread)) for t in (gate, scale, shift)
-    )
-    index_args = (0, _ext.H3A_DTYPE_I64, 0)
-    if tables:
+    branch_weight = _vector(branch_weight, columns, device, "branch_weight")
+    w_ptr = 0
+    if norm:
+        weight = _vector(weight, columns, device, "weight")
+        if weight.dtype != branch_weight.dtype:  # one dtype for both
+            weight, branch_weight = weight.float(), branch_weight.float()
+        w_ptr = weight.data_ptr()
+    gate_ptr = gate_stride = scale_ptr = scale_stride = shift_ptr = shift_stride = table_rows = 0
+    table_dtype, index_args = _ext.H3A_DTYPE_BF16, (0, _ext.H3A_DTYPE_I64, 0)
+    if norm or gate is not None:
+        if index is None:
+            raise ValueError("gate, scale and shift need an index")
+        tables = _tables([t for t in (gate, scale, shift) if t is not None], columns, device)
+        table_dtype, table_rows = _dtype(tables[0]), min([t.shape[0] for t in tables])
+        if gate is not None:
+            gate_ptr, gate_stride = tables[0].data_ptr(), tables[0].stride(0)
+        if norm:
+            scale, shift = tables[-2:]
+            scale_ptr, scale_stride, shift_ptr, shift_stride = scale.data_ptr(), scale.stride(0), shift.data_ptr(), shift.stride(0)
         index = _index(index, device)
         index_args = _index_args(index)
-    rows = residual_flat.shape[0]
-    hidden = residual_flat.new_empty((rows, columns))
-    normed = residual_flat.new_empty((rows, columns)) if weight is not None else None
+    hidden = rows_r.new_empty(shape)
+    normed = rows_r.new_empty(shape) if norm else None
     if columns:
         _ext.rmsnorm_residual_gate_rmsnorm_modulate.run(
-            device, _ext.ABI_VERSION, residual_flat.data_ptr(), branch_flat.data_ptr(), hidden.data_ptr(),
-            0 if normed is None else normed.data_ptr(), weights[0].data_ptr(), 0 if weight is None else weights[1].data_ptr(),
-            _dtype(weights[0]), gate_args[0], scale_args[0], shift_args[0],
-            _dtype(tables[0]) if tables else _ext.H3A_DTYPE_BF16, gate_args[1], scale_args[1], shift_args[1],
-            min((t.shape[0] for t in tables), default=0), *index_args, rows, columns, residual_flat.stride(0),
-            branch_flat.stride(0), hidden.stride(0), columns, float(residual_scale), float(eps),
+            device, _ext.ABI_VERSION, rows_r.data_ptr(), rows_b.data_ptr(), hidden.data_ptr(),
+            normed.data_ptr() if norm else 0, branch_weight.data_ptr(), w_ptr, _dtype(branch_weight), gate_ptr, scale_ptr,
+            shift_ptr, table_dtype, gate_stride, scale_stride, shift_stride, table_rows, *index_args, rows_r.shape[0], columns,
+            rows_r.stride(0), rows_b.stride(0), columns, columns, float(residual_scale), float(eps),
         )
-    return hidden.view(residual.shape), None if normed is None else normed.view(residual.shape)
+    return hidden, normed
 
 
 def fused_swiglu(x):

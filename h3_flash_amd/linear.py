@@ -23,10 +23,10 @@ __all__ = ["fused_linear"]
 def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
     """Rows of 16-byte chunks, as the launch reads them (else a copy)."""
 
-    size = 16 // t.element_size()
-    return t if t.stride(1) == 1 and t.stride(0) % size == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0 else (
-        t.clone(memory_format=torch.contiguous_format)
-    )
+    row, column = t.stride()
+    if column == 1 and row * t.element_size() % 16 == 0 and row >= t.shape[1] and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def fused_linear(
@@ -87,20 +87,21 @@ def fused_linear(
         gate, index = _aligned_rows(gate), _index(index, device)
         at, index_dtype, n_index = _index_args(index)
         gate_args = (gate.data_ptr(), _dtype(gate), gate.stride(0), gate.shape[0], at, index_dtype, n_index)
+    y_stride = n
     if out is None:
-        y = flat.new_empty((m, n))
-        out = y.view(shape)
+        y = out = flat.new_empty(shape)
     else:
         if out.shape != shape or out.dtype != torch.bfloat16 or out.device != device:
             raise ValueError(f"out must be a bf16 {shape} tensor on {device}")
         y = out.view(-1, n) if m else out.new_empty((0, n))
         if m and (y.stride(1) != 1 or y.stride(0) % 8 or y.stride(0) < n or y.data_ptr() % 16):
             raise ValueError("out must have contiguous, 16-byte aligned rows")
+        y_stride = y.stride(0)
     if m:
         args = (
             _ext.ABI_VERSION, flat.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(),
             _ext.H3A_DTYPE_BF16 if bias is None else _dtype(bias), 0 if residual is None else residual.data_ptr(), *gate_args,
-            y.data_ptr(), m, k, n, flat.stride(0), weight.stride(0), 0 if residual is None else residual.stride(0), y.stride(0),
+            y.data_ptr(), m, k, n, flat.stride(0), weight.stride(0), 0 if residual is None else residual.stride(0), y_stride,
             _ext.ACTIVATIONS[activation], int(gated),
         )
         rc = _ext.linear(device, *args, 0, _ext.H3A_WORKSPACE_ASK)

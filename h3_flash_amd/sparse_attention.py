@@ -29,6 +29,12 @@ def _blocks(n: int, size: int) -> int:
     return -(-n // size)
 
 
+def _select_workspace(heads: int, nq: int, nk: int) -> int:
+    """h3a_block_select_workspace_size without the call: the means and scores."""
+
+    return sum(-(-heads * n // 256) * 256 for n in (nq * 512, nk * 512, nq * nk * 4))
+
+
 def _check_pair(q: torch.Tensor, k: torch.Tensor) -> None:
     if q.shape[3] != HEAD_DIM:
         raise ValueError(f"head_dim must be {HEAD_DIM}, got {q.shape[3]}")
@@ -73,9 +79,7 @@ def select_key_blocks(
         _ext.ABI_VERSION, q.data_ptr(), k.data_ptr(), 0 if always is None else always.data_ptr(), index.data_ptr(),
         B, H, Sq, k.shape[1], D, *_strides3(q), *_strides3(k), topk,
     )
-    need = _ext.block_select_workspace_size(device, *args, 0, 0)
-    if need < 0:
-        _ext.check(_ext.load_library(), need)
+    need = _select_workspace(B * H, nq, nk)
     workspace = torch.empty(need, dtype=torch.uint8, device=device)
     _ext.block_select.run(device, *args, workspace.data_ptr(), need)
     return index

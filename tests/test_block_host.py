@@ -16,6 +16,7 @@ import torch
 
 from h3_flash_amd import _ext, fused_linear, select_key_blocks, sparse_attn_func
 from h3_flash_amd.fusions import fused_rmsnorm_residual_gate_rmsnorm_modulate
+from h3_flash_amd.sparse_attention import _select_workspace
 
 ROOT = Path(__file__).resolve().parents[1]
 HEADER = ROOT / "include" / "h3block.h"
@@ -208,6 +209,14 @@ def test_null_arguments_and_empty_problems(lib):
     # 2 heads: 2 query and 5 key blocks of 512-byte means, 2 x 5 scores, each part 256-byte aligned
     assert lib.h3a_block_select_workspace_size(ctypes.byref(_select())) == 2048 + 5120 + 256
     assert lib.h3a_attn_sparse_workspace_size(ctypes.byref(_sparse(max_blocks=8000))) == UNSUPPORTED
+
+
+@host_only
+@pytest.mark.parametrize("batch, heads, sq, sk", [(1, 1, 1, 1), (2, 3, 257, 65), (1, 40, 1560, 1560), (1, 5, 49920, 129024)])
+def test_selection_workspace_of_the_wrapper(lib, batch, heads, sq, sk):
+    args = _select(batch=batch, heads=heads, seqlen_q=sq, seqlen_k=sk, topk=1)
+    want = lib.h3a_block_select_workspace_size(ctypes.byref(args))
+    assert _select_workspace(batch * heads, -(-sq // 256), -(-sk // 64)) == want
 
 
 def test_host_tensors_never_reach_a_launch():
