@@ -311,24 +311,28 @@ hipError_t launch_tile(const LinearParams& p, hipStream_t stream) {
     return p.gated ? launch_tile_t<TF, NT, SW, SX, true>(p, stream) : launch_tile_t<TF, NT, SW, SX, false>(p, stream);
 }
 
-// The tile shapes, with the time of a K step of 64 and a tile's fixed part
-// (launch, first loads, epilogue). Fitted to graph replays of 22 sizes (64 to
-// 12,480 tokens, 1,024 to 32,256 features, k 1,024 to 14,336) in every shape and
-// split; the choice by them takes 1.2% longer than the best of all, in the mean.
+// The tile shapes, with the time of a K step of 64 with all CUs busy and a tile's
+// fixed part (launch, first loads, epilogue). Fitted to graph replays of 25 sizes
+// (40 to 12,480 tokens, 1,024 to 32,256 features, k 1,024 to 14,336) in every shape
+// and split; the choice by them takes 1.5% longer than the best of all, in the
+// mean. (Up to 128 features a K step is bound by what the L2s deliver: 32 KB per
+// CU at 128 x 128, 21 TB/s over the chip.)
 struct Shape {
     int tf, nt;
     float step_us, fixed_us;
     hipError_t (*launch)(const LinearParams&, hipStream_t);
 };
 constexpr Shape kShapes[] = {
-    {256, 16, 1.44f, 4.4f, launch_tile<256, 16, 3, 2>}, {256, 12, 1.14f, 5.1f, launch_tile<256, 12, 3, 2>},
-    {256, 8, 0.81f, 7.4f, launch_tile<256, 8, 4, 2>},   {128, 8, 0.50f, 4.9f, launch_tile<128, 8, 6, 4>},
-    {128, 4, 0.34f, 3.5f, launch_tile<128, 4, 7, 5>},
+    {256, 16, 1.42f, 10.0f, launch_tile<256, 16, 3, 2>}, {256, 12, 1.10f, 9.5f, launch_tile<256, 12, 3, 2>},
+    {256, 8, 0.82f, 8.7f, launch_tile<256, 8, 4, 2>},    {128, 8, 0.50f, 5.8f, launch_tile<128, 8, 6, 4>},
+    {128, 6, 0.40f, 5.8f, launch_tile<128, 6, 7, 4>},    {128, 4, 0.34f, 4.9f, launch_tile<128, 4, 7, 5>},
+    {128, 2, 0.27f, 3.5f, launch_tile<128, 2, 8, 6>},
 };
-// A second launch joins the pieces, over their sums at 0.38 us a MB.
-constexpr float kJoinUs = 5.4f, kJoinUsPerByte = 0.38e-6f;
+constexpr float kIdleGain = 0.35f;  // of a K step's time, saved as the CUs of a round go idle
+// A second launch joins the pieces, over their sums at 0.32 us a MB.
+constexpr float kJoinUs = 5.8f, kJoinUsPerByte = 0.32e-6f;
 constexpr int kSplits[] = {2, 3, 4, 6, 8};
-constexpr int kMinPieceSteps = 8;
+constexpr int kMinPieceSteps = 16;
 
 // ---------------------------------------------------------------- few tokens
 
@@ -452,17 +456,21 @@ void plan_linear(LinearParams& p, int cus, int64_t* workspace) {
         const int to = p.gated ? s.tf / 2 : s.tf, tokens = 16 * s.nt;
         const int64_t n_tiles = (p.n + to - 1) / to, m_tiles = (p.m + tokens - 1) / tokens, tiles = n_tiles * m_tiles;
         if (tiles >= ((int64_t)1 << 31)) continue;
-        // Whole: rounds of tiles over the CUs; past six rounds the tiles no longer
-        // run in step, and the last round costs about half of one.
+        // Whole: rounds of tiles over the CUs, the last one faster the fewer CUs it
+        // keeps busy; past six rounds the tiles no longer run in step, and the
+        // last round costs about half of one.
         const int64_t full = tiles / cus * cus, rest = tiles - full;
         const float tile_us = (float)steps * s.step_us + s.fixed_us, rounds = (float)tiles / (float)cus;
-        float us = (rounds <= 6.f ? ceilf(rounds) : rounds + 0.5f) * tile_us;
+        auto last_us = [&](int n) {
+            return (float)steps / (float)n * s.step_us * (1.f - kIdleGain * (1.f - (float)(rest * n) / (float)cus)) + s.fixed_us;
+        };
+        float us = rounds > 6.f ? (rounds + 0.5f) * tile_us : (float)(full / cus) * tile_us + (rest > 0 ? last_us(1) : 0.f);
         int split = 1;
-        // The last round in pieces, at most one per CU.
+        // The last round in pieces, at most one per CU (of the smallest tiles none:
+        // they serve short reductions).
         for (const int n : kSplits) {
-            if (rest == 0 || rest * n > cus || steps / n < kMinPieceSteps) break;
-            const float cut = (float)(full / cus) * tile_us + (float)steps / (float)n * s.step_us + s.fixed_us + kJoinUs +
-                              (float)(rest * n * s.tf * tokens * 4) * kJoinUsPerByte;
+            if (rest == 0 || rest * n > cus || steps / n < kMinPieceSteps || s.nt == 2) break;
+            const float cut = (float)(full / cus) * tile_us + last_us(n) + kJoinUs + (float)(rest * n * s.tf * tokens * 4) * kJoinUsPerByte;
             if (cut < us) {
                 us = cut;
                 split = n;

@@ -46,6 +46,36 @@ CASES = [
     (1297, 1544, 2056, "gelu_tanh", False, F32, True, F32),
     (1560, 5120, 1288, "silu", True, BF16, True, BF16),
     (2500, 2048, 4096, None, False, None, True, BF16),
+    # few tokens over wide weights: two and four blocks of rows per workgroup
+    (5, 72, 4104, "relu", False, BF16, True, None),
+    (20, 200, 4104, "gelu", False, F32, True, BF16),
+    (16, 72, 16408, None, False, BF16, True, F32),
+    (32, 264, 16392, "silu", False, None, False, None),
+    (3, 136, 8200, "silu", True, F32, True, BF16),
+    (27, 136, 8200, "gelu_tanh", True, BF16, False, None),
+    # every tile shape, plain and gated
+    (200, 264, 8200, "relu", False, BF16, True, None),
+    (300, 264, 8200, None, False, F32, True, BF16),
+    (450, 264, 8200, "silu", False, None, True, None),
+    (800, 264, 14344, "gelu", False, BF16, True, F32),
+    (70, 264, 8200, "gelu", True, BF16, True, None),
+    (100, 264, 8200, "silu", True, None, True, F32),
+    (150, 264, 8200, "relu", True, F32, False, None),
+    (600, 264, 8200, "silu", True, BF16, True, BF16),
+    (1100, 264, 14344, None, True, None, False, None),
+    # tiles in pieces along k: alone, and after rounds of whole tiles; k ends
+    # inside the last piece's last step
+    (40, 4104, 264, "gelu_tanh", False, BF16, True, BF16),
+    (40, 4104, 264, "silu", True, F32, True, F32),
+    (70, 8200, 2696, None, False, BF16, False, None),
+    (70, 8200, 1032, "gelu", True, None, True, None),
+    (100, 8200, 4104, "relu", False, F32, True, BF16),
+    (200, 8200, 1032, "silu", True, BF16, False, None),
+    (150, 4104, 8200, "silu", True, None, True, BF16),
+    (450, 8200, 8200, None, False, BF16, True, F32),
+    (450, 8200, 8200, "silu", True, None, False, None),
+    (3120, 4104, 2696, "gelu", True, BF16, True, BF16),
+    (3120, 14344, 5368, None, False, F32, True, BF16),
 ]
 
 
