@@ -347,7 +347,7 @@ constexpr int kRowsMaxTokens = 32;
 template <int NA, int NB, bool kGated>
 __global__ __launch_bounds__(NA == 1 ? 1024 : 512) void linear_rows_kernel(LinearParams p) {
     constexpr int kS = kGated ? 2 : 1, NF = NA / kS;  // blocks of output features
-    constexpr int kU = NA * NB >= 4 ? 2 : 4;
+    constexpr int kU = NA * NB >= 4 ? 1 : 4;
     extern __shared__ f32x4 part[];  // [wave][NA * NB][64]
     const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, l15 = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = (int)blockDim.x >> 6;

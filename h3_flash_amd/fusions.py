@@ -44,6 +44,16 @@ def _rows(x: torch.Tensor, name: str, columns: int) -> torch.Tensor:
     return flat if flat.stride(1) == 1 else flat.contiguous()
 
 
+def _row_span(x: torch.Tensor, name: str, columns: int) -> tuple[torch.Tensor, int, int]:
+    """The tensor that holds x's rows as :func:`_rows` gives them, their number and
+    stride (a contiguous x as it is: no view is made of it)."""
+
+    if x.is_contiguous() and x.dtype == torch.bfloat16 and x.is_cuda and columns:
+        return x, x.numel() // columns, columns
+    flat = _rows(x, name, columns)
+    return flat, flat.shape[0], flat.stride(0)
+
+
 def _vector(t: torch.Tensor, columns: int, device: torch.device, name: str) -> torch.Tensor:
     if t.shape != (columns,):
         if t.shape[-1] != columns or t.numel() != columns:
@@ -160,7 +170,8 @@ def fused_rmsnorm_residual_gate_rmsnorm_modulate(
     if norm != (scale is not None) or norm != (shift is not None):
         raise ValueError("weight, scale and shift go together: give all three or none")
     device = residual.device
-    rows_r, rows_b = _rows(residual, "residual", columns), _rows(branch, "branch", columns)
+    rows_r, n_rows, stride_r = _row_span(residual, "residual", columns)
+    rows_b, _, stride_b = _row_span(branch, "branch", columns)
     if branch.device != device:
         raise ValueError(f"residual and branch must be on one device, got {device} and {branch.device}")
     branch_weight = _vector(branch_weight, columns, device, "branch_weight")
@@ -184,14 +195,14 @@ def fused_rmsnorm_residual_gate_rmsnorm_modulate(
             scale_ptr, scale_stride, shift_ptr, shift_stride = scale.data_ptr(), scale.stride(0), shift.data_ptr(), shift.stride(0)
         index = _index(index, device)
         index_args = _index_args(index)
-    hidden = rows_r.new_empty(shape)
-    normed = rows_r.new_empty(shape) if norm else None
+    hidden = torch.empty_like(residual, memory_format=torch.contiguous_format)
+    normed = torch.empty_like(hidden) if norm else None
     if columns:
         _ext.rmsnorm_residual_gate_rmsnorm_modulate.run(
             device, _ext.ABI_VERSION, rows_r.data_ptr(), rows_b.data_ptr(), hidden.data_ptr(),
             normed.data_ptr() if norm else 0, branch_weight.data_ptr(), w_ptr, _dtype(branch_weight), gate_ptr, scale_ptr,
-            shift_ptr, table_dtype, gate_stride, scale_stride, shift_stride, table_rows, *index_args, rows_r.shape[0], columns,
-            rows_r.stride(0), rows_b.stride(0), columns, columns, float(residual_scale), float(eps),
+            shift_ptr, table_dtype, gate_stride, scale_stride, shift_stride, table_rows, *index_args, n_rows, columns,
+            stride_r, stride_b, columns, columns, float(residual_scale), float(eps),
         )
     return hidden, normed
 

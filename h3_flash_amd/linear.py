@@ -15,7 +15,7 @@ from __future__ import annotations
 import torch
 
 from . import _ext
-from .fusions import _dtype, _index, _index_args, _rows, _tables, _vector
+from .fusions import _dtype, _index, _index_args, _row_span, _rows, _tables, _vector
 
 __all__ = ["fused_linear"]
 
@@ -27,6 +27,16 @@ def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
     if column == 1 and row * t.element_size() % 16 == 0 and row >= t.shape[1] and t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
+
+
+def _operand(x: torch.Tensor, name: str, columns: int) -> tuple[torch.Tensor, int, int]:
+    """Rows of 16-byte chunks: the tensor that holds them, their number and stride."""
+
+    held, rows, stride = _row_span(x, name, columns)
+    if stride % 8 or stride < columns or held.data_ptr() % 16:
+        held = _aligned_rows(_rows(held, name, columns))
+        stride = held.stride(0)
+    return held, rows, stride
 
 
 def fused_linear(
@@ -64,21 +74,21 @@ def fused_linear(
     n = rows // 2 if gated else rows
     if k % 8 or n % 8 or k == 0 or n == 0:
         raise ValueError(f"k and n must be positive multiples of 8, got {k} and {n}")
-    flat = _aligned_rows(_rows(x, "x", k))
-    device, m = x.device, flat.shape[0]
+    flat, m, x_stride = _operand(x, "x", k)
+    device = x.device
     if weight.device != device:
         raise ValueError(f"x and weight must be on one device, got {device} and {weight.device}")
     weight = _aligned_rows(weight)
     if bias is not None:
         bias = _vector(bias, rows, device, "bias")
         bias = bias if bias.data_ptr() % 16 == 0 else bias.clone()
-    shape = (*x.shape[:-1], n)
+    shape, residual_stride = (*x.shape[:-1], n), 0
     if residual is not None:
         if residual.shape != shape:
             raise ValueError(f"residual must be {shape}, got {tuple(residual.shape)}")
         if residual.device != device:
             raise ValueError(f"x and residual must be on one device, got {device} and {residual.device}")
-        residual = _aligned_rows(_rows(residual, "residual", n))
+        residual, _, residual_stride = _operand(residual, "residual", n)
     gate_args = (0, _ext.H3A_DTYPE_BF16, 0, 0, 0, _ext.H3A_DTYPE_I64, 0)
     if gate is not None:
         if index is None:
@@ -101,7 +111,7 @@ def fused_linear(
         args = (
             _ext.ABI_VERSION, flat.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(),
             _ext.H3A_DTYPE_BF16 if bias is None else _dtype(bias), 0 if residual is None else residual.data_ptr(), *gate_args,
-            y.data_ptr(), m, k, n, flat.stride(0), weight.stride(0), 0 if residual is None else residual.stride(0), y_stride,
+            y.data_ptr(), m, k, n, x_stride, weight.stride(0), residual_stride, y_stride,
             _ext.ACTIVATIONS[activation], int(gated),
         )
         rc = _ext.linear(device, *args, 0, _ext.H3A_WORKSPACE_ASK)
