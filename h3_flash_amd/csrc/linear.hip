@@ -267,7 +267,11 @@ __global__ __launch_bounds__(kPThreads, 1) void linear_kernel(LinearParams p) {
         for (int b = 0; b < T::NB; ++b) out[(a * T::NB + b) * kPThreads] = acc[a][b];
 }
 
-// Workgroup (i, a): feature block a of every wave of split tile i.
+// Workgroup (i, a, b): blocks (a, b) of every wave of split tile i, the pieces' sums
+// all in flight before they are added. (All token blocks in one workgroup: 24 us
+// for 13 tiles of 256 x 256 in 8 pieces, now 7.)
+constexpr int kMaxSplit = 8;
+
 template <int TF, int NT, int SW, int SX, bool kGated>
 __global__ __launch_bounds__(kPThreads) void linear_join_kernel(LinearParams p) {
     using T = Tile<TF, NT, SW, SX>;
@@ -278,19 +282,25 @@ __global__ __launch_bounds__(kPThreads) void linear_join_kernel(LinearParams p) 
     const int f = tc.f0 + 16 * (NF * wn + a) + 4 * (lane >> 4);
     const f32x4* const in = (const f32x4*)p.ws + (int64_t)blockIdx.x * (T::NA * T::NB * kPThreads) + tid;
     const int64_t step = (int64_t)rest * (T::NA * T::NB * kPThreads);
-    if (f >= p.n) return;
+    const int b = blockIdx.z, m = tc.m0 + 16 * (T::NB * wm + b) + (lane & 15);
+    if (f >= p.n || m >= p.m) return;
+    f32x4 part[kMaxSplit][kS];
 #pragma unroll
-    for (int b = 0; b < T::NB; ++b) {
-        const int m = tc.m0 + 16 * (T::NB * wm + b) + (lane & 15);
-        if (m >= p.m) continue;
-        f32x4 z[kS];
+    for (int c = 0; c < kMaxSplit; ++c) {
+        if (c >= p.split) break;
 #pragma unroll
-        for (int s = 0; s < kS; ++s) z[s] = f32x4{};
-        for (int c = 0; c < p.split; ++c)
-#pragma unroll
-            for (int s = 0; s < kS; ++s) z[s] += in[c * step + ((kS * a + s) * T::NB + b) * kPThreads];
-        finish4<kS>(p, z, m, f);
+        for (int s = 0; s < kS; ++s) part[c][s] = in[c * step + ((kS * a + s) * T::NB + b) * kPThreads];
     }
+    f32x4 z[kS];
+#pragma unroll
+    for (int s = 0; s < kS; ++s) z[s] = f32x4{};
+#pragma unroll
+    for (int c = 0; c < kMaxSplit; ++c) {
+        if (c >= p.split) break;
+#pragma unroll
+        for (int s = 0; s < kS; ++s) z[s] += part[c][s];
+    }
+    finish4<kS>(p, z, m, f);
 }
 
 template <int TF, int NT, int SW, int SX, bool kGated>
@@ -301,8 +311,8 @@ hipError_t launch_tile_t(const LinearParams& p, hipStream_t stream) {
     hipLaunchKernelGGL((linear_kernel<TF, NT, SW, SX, kGated>), grid, dim3(kPThreads), 0, stream, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || rest == 0) return e;
-    hipLaunchKernelGGL((linear_join_kernel<TF, NT, SW, SX, kGated>), dim3((unsigned)rest, T::NA / (kGated ? 2 : 1)), dim3(kPThreads), 0,
-                       stream, p);
+    hipLaunchKernelGGL((linear_join_kernel<TF, NT, SW, SX, kGated>), dim3((unsigned)rest, T::NA / (kGated ? 2 : 1), T::NB),
+                       dim3(kPThreads), 0, stream, p);
     return hipGetLastError();
 }
 
@@ -314,7 +324,7 @@ hipError_t launch_tile(const LinearParams& p, hipStream_t stream) {
 // The tile shapes, with the time of a K step of 64 with all CUs busy and a tile's
 // fixed part (launch, first loads, epilogue). Fitted to graph replays of 25 sizes
 // (40 to 12,480 tokens, 1,024 to 32,256 features, k 1,024 to 14,336) in every shape
-// and split; the choice by them takes 1.5% longer than the best of all, in the
+// and split; the choice by them takes 0.3% longer than the best of all, in the
 // mean. (Up to 128 features a K step is bound by what the L2s deliver: 32 KB per
 // CU at 128 x 128, 21 TB/s over the chip.)
 struct Shape {
@@ -323,15 +333,15 @@ struct Shape {
     hipError_t (*launch)(const LinearParams&, hipStream_t);
 };
 constexpr Shape kShapes[] = {
-    {256, 16, 1.42f, 10.0f, launch_tile<256, 16, 3, 2>}, {256, 12, 1.10f, 9.5f, launch_tile<256, 12, 3, 2>},
-    {256, 8, 0.82f, 8.7f, launch_tile<256, 8, 4, 2>},    {128, 8, 0.50f, 5.8f, launch_tile<128, 8, 6, 4>},
-    {128, 6, 0.40f, 5.8f, launch_tile<128, 6, 7, 4>},    {128, 4, 0.34f, 4.9f, launch_tile<128, 4, 7, 5>},
-    {128, 2, 0.27f, 3.5f, launch_tile<128, 2, 8, 6>},
+    {256, 16, 1.36f, 13.3f, launch_tile<256, 16, 3, 2>}, {256, 12, 1.05f, 11.8f, launch_tile<256, 12, 3, 2>},
+    {256, 8, 0.80f, 9.3f, launch_tile<256, 8, 4, 2>},    {128, 8, 0.50f, 5.9f, launch_tile<128, 8, 6, 4>},
+    {128, 6, 0.40f, 5.9f, launch_tile<128, 6, 7, 4>},    {128, 4, 0.34f, 5.3f, launch_tile<128, 4, 7, 5>},
+    {128, 2, 0.27f, 3.6f, launch_tile<128, 2, 8, 6>},
 };
-constexpr float kIdleGain = 0.35f;  // of a K step's time, saved as the CUs of a round go idle
+constexpr float kIdleGain = 0.36f;  // of a K step's time, saved as the CUs of a round go idle
 // A second launch joins the pieces, over their sums at 0.32 us a MB.
-constexpr float kJoinUs = 5.8f, kJoinUsPerByte = 0.32e-6f;
-constexpr int kSplits[] = {2, 3, 4, 6, 8};
+constexpr float kJoinUs = 1.9f, kJoinUsPerByte = 0.32e-6f;
+constexpr int kSplits[] = {2, 3, 4, 6, kMaxSplit};
 constexpr int kMinPieceSteps = 16;
 
 // ---------------------------------------------------------------- few tokens

@@ -76,6 +76,11 @@ CASES = [
     (450, 8200, 8200, "silu", True, None, False, None),
     (3120, 4104, 2696, "gelu", True, BF16, True, BF16),
     (3120, 14344, 5368, None, False, F32, True, BF16),
+    (3120, 4104, 8200, "silu", True, None, False, None),
+    (4100, 8200, 1032, "relu", False, BF16, True, None),
+    (1560, 14336, 5376, None, False, BF16, True, BF16),
+    (100, 264, 8200, "gelu_tanh", False, None, True, F32),
+    (40, 264, 8200, None, True, BF16, True, None),
 ]
 
 
