@@ -491,7 +491,12 @@ void plan_linear(LinearParams& p, int cus, int64_t* workspace) {
         p.shape = i;
         p.m_tiles = (int32_t)m_tiles;
         p.n_tiles = (int32_t)n_tiles;
-        const int group_tokens = p.m <= 2048 ? 2048 : p.m <= 16384 ? 1024 : 768;
+        // Tokens of a group of the tile order: each group reads all of w from HBM
+        // (us at 256 tokens a tile, groups of 2 / 4 / 6 / 8 / 12 / 25: 6,240 x 5,376 x
+        // 28,672 1,461 / 1,397 / 1,361 / 1,379 / 1,374 / 1,407; 6,240 x 14,336 x
+        // 5,376 720 / 712 / 711 / 711 / 713 / 737; of 2 / 3 / 4 / 6 / 8: 24,960 x
+        // 5,120 x 15,360 2,826 / 2,799 / 2,838 / 2,986 / 2,997).
+        const int group_tokens = p.m <= 2048 ? 2048 : p.m <= 16384 ? 1536 : 768;
         p.group_m = (int32_t)(group_tokens / tokens < m_tiles ? group_tokens / tokens : m_tiles);
         p.split = split;
         p.n_full = (int32_t)(split > 1 ? full : tiles);
