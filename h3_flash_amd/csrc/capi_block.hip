@@ -64,8 +64,11 @@ int prepare_select(const h3a_block_select_args* a, h3a::SelectParams& p, int64_t
         return fail(H3A_EINVAL, "%s: topk must be in [1, %lld], got %lld", fn, (long long)nk, (long long)a->topk);
     if (nk > h3a::select_max_blocks())
         return fail(H3A_EUNSUPPORTED, "%s: at most %d key blocks, got %lld", fn, h3a::select_max_blocks(), (long long)nk);
-    if ((__int128)a->batch * a->heads > 65535 || (__int128)a->batch * a->heads * (nq + nk) > INT32_MAX)
-        return fail(H3A_EUNSUPPORTED, "%s: batch x heads must be at most 65535, and with the blocks below 2^31", fn);
+    // (Work items of the three launches: 256 per block, 256 per 16 x 128 scores of
+    // a head, at most 1,024 per query block.)
+    if ((__int128)a->batch * a->heads > 65535 || (__int128)a->batch * a->heads * (nq + nk) >= ((int64_t)1 << 22) ||
+        ((nq + 15) / 16) * ((nk + 127) / 128) >= ((int64_t)1 << 24))
+        return fail(H3A_EUNSUPPORTED, "%s: batch x heads must be at most 65535, and with the blocks below 2^22", fn);
     if ((rc = check_view(fn, "q", a->q, a->q_stride, 1)) != H3A_OK) return rc;
     if ((rc = check_view(fn, "k", a->k, a->k_stride, 1)) != H3A_OK) return rc;
     if (!a->index || !aligned4(a->index)) return fail(H3A_EINVAL, "%s: index must be a 4-byte aligned device pointer", fn);
@@ -120,7 +123,8 @@ int prepare_sparse(const h3a_attn_sparse_args* a, h3a::SparseParams& p, int64_t*
         return fail(H3A_EINVAL, "%s: lse must be 4-byte aligned with non-negative strides", fn);
     const int64_t nq = (a->seqlen_q + H3A_BLOCK_Q - 1) / H3A_BLOCK_Q;
     const __int128 tiles = (__int128)a->batch * a->heads * nq;
-    if (tiles > INT32_MAX / 64) return fail(H3A_EUNSUPPORTED, "%s: grid too large", fn);
+    // (512 work items for each of a tile's 8 units: 2^32 a launch.)
+    if (tiles >= ((int64_t)1 << 20)) return fail(H3A_EUNSUPPORTED, "%s: grid too large", fn);
     p.q = a->q; p.k = a->k; p.v = a->v; p.o = a->o; p.lse = a->lse;
     p.q_sb = a->q_stride[0]; p.q_sh = a->q_stride[2]; p.q_rs = (int32_t)(a->q_stride[1] * 2);
     p.k_sb = a->k_stride[0]; p.k_sh = a->k_stride[2]; p.k_rs = (int32_t)(a->k_stride[1] * 2);
@@ -204,6 +208,7 @@ int prepare_linear(const h3a_linear_args* a, h3a::LinearParams& p, int64_t* need
     p.m = (int32_t)a->m; p.k = (int32_t)a->k; p.n = (int32_t)a->n;
     p.act = a->activation; p.gated = a->gated != 0;
     h3a::plan_linear(p, h3a::device_cus(), need);
+    if (p.shape < -1) return fail(H3A_EUNSUPPORTED, "%s: grid too large", fn);
     return H3A_OK;
 }
 
@@ -249,7 +254,8 @@ int h3a_rmsnorm_residual_gate_rmsnorm_modulate(const h3a_rmsnorm_residual_gate_r
     if (a->abi_version != H3A_ABI_VERSION)
         return fail(H3A_EINVAL, "%s: abi_version %d, library is %d", fn, a->abi_version, H3A_ABI_VERSION);
     if (a->rows < 0 || a->cols <= 0) return fail(H3A_EINVAL, "%s: bad extents (rows=%lld cols=%lld)", fn, (long long)a->rows, (long long)a->cols);
-    if (a->rows >= ((int64_t)1 << 31) || a->cols >= ((int64_t)1 << 30)) return fail(H3A_EUNSUPPORTED, "%s: extents too large", fn);
+    // (A workgroup of 256 per row: 2^32 work items a launch.)
+    if (a->rows >= ((int64_t)1 << 24) || a->cols >= ((int64_t)1 << 30)) return fail(H3A_EUNSUPPORTED, "%s: extents too large", fn);
     if (!(a->eps >= 0.f) || !isfinite(a->eps)) return fail(H3A_EINVAL, "%s: eps must be finite and not negative", fn);
     if (!isfinite(a->residual_scale)) return fail(H3A_EINVAL, "%s: residual_scale must be finite", fn);
     if (!bf16_or_f32(a->w_dtype)) return fail(H3A_EINVAL, "%s: unknown weight dtype %d", fn, a->w_dtype);

@@ -353,6 +353,7 @@ constexpr int kMinPieceSteps = 16;
 // rows, from the caches, once per NA blocks. The waves' partial sums meet in
 // LDS, in wave order.
 constexpr int kRowsMaxTokens = 32;
+constexpr int kRowsForm = -1, kNoForm = -2;  // in place of a tile shape
 
 template <int NA, int NB, bool kGated>
 __global__ __launch_bounds__(NA == 1 ? 1024 : 512) void linear_rows_kernel(LinearParams p) {
@@ -457,15 +458,16 @@ hipError_t launch_rows(const LinearParams& p, int cus, hipStream_t stream) {
 void plan_linear(LinearParams& p, int cus, int64_t* workspace) {
     if (cus <= 0) cus = 256;
     *workspace = 0;
-    p.shape = -1;
+    p.shape = kRowsForm;
     if (p.m <= kRowsMaxTokens) return;
+    p.shape = kNoForm;
     const int steps = (p.k + kPK - 1) / kPK;
     float best_us = 0.f;
     for (int i = 0; i < (int)(sizeof(kShapes) / sizeof(kShapes[0])); ++i) {
         const Shape& s = kShapes[i];
         const int to = p.gated ? s.tf / 2 : s.tf, tokens = 16 * s.nt;
         const int64_t n_tiles = (p.n + to - 1) / to, m_tiles = (p.m + tokens - 1) / tokens, tiles = n_tiles * m_tiles;
-        if (tiles >= ((int64_t)1 << 31)) continue;
+        if (tiles * kPThreads > UINT32_MAX) continue;  // work items of a launch
         // Whole: rounds of tiles over the CUs, the last one faster the fewer CUs it
         // keeps busy; past six rounds the tiles no longer run in step, and the
         // last round costs about half of one.
@@ -505,6 +507,7 @@ void plan_linear(LinearParams& p, int cus, int64_t* workspace) {
 }
 
 hipError_t launch_linear(const LinearParams& p, int cus, hipStream_t stream) {
+    if (p.shape == kNoForm) return hipErrorInvalidConfiguration;
     if (p.shape >= 0) return kShapes[p.shape].launch(p, stream);
     if (p.m <= 16) return launch_rows<1>(p, cus, stream);
     return launch_rows<2>(p, cus, stream);

@@ -142,6 +142,7 @@ INVALID, UNSUPPORTED = _ext.H3A_EINVAL, _ext.H3A_EUNSUPPORTED
         ("h3a_linear", _linear(y_stride=36), INVALID, "strides"),
         ("h3a_linear", _linear(weight_stride=1 << 23), UNSUPPORTED, "2^31"),
         ("h3a_linear", _linear(m=1 << 31), UNSUPPORTED, "too large"),
+        ("h3a_linear", _linear(m=1 << 30, n=1 << 14, y_stride=1 << 14), UNSUPPORTED, "grid too large"),
         ("h3a_linear", _linear(bias=P, bias_dtype=2), INVALID, "bias dtype"),
         ("h3a_linear", _linear(bias=P + 8), INVALID, "bias"),
         ("h3a_linear", _linear(residual=P, residual_stride=24), INVALID, "residual_stride"),
@@ -151,6 +152,7 @@ INVALID, UNSUPPORTED = _ext.H3A_EINVAL, _ext.H3A_EUNSUPPORTED
         ("h3a_linear", _linear(gate=P, gate_stride=36, table_rows=1, index=P, index_dtype=3, n_index=1), INVALID, "gate rows"),
         ("h3a_rmsnorm_residual_gate_rmsnorm_modulate", _norm(abi_version=0), INVALID, "abi_version"),
         ("h3a_rmsnorm_residual_gate_rmsnorm_modulate", _norm(cols=0), INVALID, "bad extents"),
+        ("h3a_rmsnorm_residual_gate_rmsnorm_modulate", _norm(rows=1 << 24), UNSUPPORTED, "too large"),
         ("h3a_rmsnorm_residual_gate_rmsnorm_modulate", _norm(eps=-1.0), INVALID, "eps"),
         ("h3a_rmsnorm_residual_gate_rmsnorm_modulate", _norm(residual_scale=float("nan")), INVALID, "residual_scale"),
         ("h3a_rmsnorm_residual_gate_rmsnorm_modulate", _norm(w_dtype=2), INVALID, "weight dtype"),
@@ -170,6 +172,8 @@ INVALID, UNSUPPORTED = _ext.H3A_EINVAL, _ext.H3A_EUNSUPPORTED
         ("h3a_block_select", _select(topk=6), INVALID, "topk"),
         ("h3a_block_select", _select(seqlen_k=64 * 32768 + 1), UNSUPPORTED, "key blocks"),
         ("h3a_block_select", _select(batch=70000), UNSUPPORTED, "65535"),
+        ("h3a_block_select", _select(seqlen_q=1 << 29, seqlen_k=64 * 32768, batch=3), UNSUPPORTED, "2^22"),
+        ("h3a_block_select", _select(seqlen_q=1 << 29, seqlen_k=64 * 32768), UNSUPPORTED, "2^22"),
         ("h3a_block_select", _select(q_stride=(0, 100, 128)), INVALID, "q strides"),
         ("h3a_block_select", _select(k=P + 4), INVALID, "k must"),
         ("h3a_block_select", _select(index=0), INVALID, "index"),
@@ -190,6 +194,7 @@ INVALID, UNSUPPORTED = _ext.H3A_EINVAL, _ext.H3A_EUNSUPPORTED
         ("h3a_attn_sparse", _sparse(block_count=P + 2), INVALID, "block_count"),
         ("h3a_attn_sparse", _sparse(lse=P + 2), INVALID, "lse"),
         ("h3a_attn_sparse", _sparse(seqlen_q=1 << 30), INVALID, "too large"),
+        ("h3a_attn_sparse", _sparse(seqlen_q=1 << 28), UNSUPPORTED, "grid too large"),
     ],
 )
 def test_validation(lib, name, args, code, message):
@@ -230,3 +235,31 @@ def test_host_tensors_never_reach_a_launch():
     ):
         with pytest.raises((RuntimeError, ValueError), match="ROCm device"):
             call()
+
+
+def test_sparse_kernels_fit_and_use_every_untracked_load(tmp_path):
+    """The forms over lists, as tests/test_kernel_resources.py asks of the dense
+    ones: a workgroup per CU, no load left in flight in registers that no path
+    ahead reads."""
+
+    resources = pytest.importorskip("test_kernel_resources")
+    if not resources.LIB_PATH.is_file():
+        pytest.skip("library not built")
+    found = 0
+    for i, co in enumerate(resources.gfx950_code_objects(resources.LIB_PATH.read_bytes())):
+        path = tmp_path / f"{i}.co"
+        for k in resources.kernel_metadata(co):
+            name = k[".name"]
+            if "attn_sparse" not in name:
+                continue
+            found += 1
+            assert k[".vgpr_count"] + k.get(".agpr_count", 0) <= 256 and k[".max_flat_workgroup_size"] == 512, name
+            assert k[".group_segment_fixed_size"] <= 160 * 1024 and k[".private_segment_fixed_size"] == 0, name
+            if resources._objdump() is None:
+                continue
+            path.write_bytes(co)
+            asm = subprocess.run([resources._objdump(), "-d", f"--disassemble-symbols={name}", str(path)], check=True,
+                                 capture_output=True, text=True).stdout
+            assert "buffer_load_dwordx4" in asm
+            assert resources._unused_loads(asm) == [], name
+    assert found == 2
