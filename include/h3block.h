@@ -129,7 +129,8 @@ H3A_API int h3a_rmsnorm_residual_gate_rmsnorm_modulate(const h3a_rmsnorm_residua
  * scores are taken from the lowest index on.
  * q and k are bf16 (batch, seq, head) views as for h3a_attn_fwd; always is
  * (nk,) bytes or NULL; index is contiguous int32 (batch, heads, nq, topk) with
- * 1 <= topk <= nk (none is written when nq or nk is 0). nk is at most 32,768.
+ * 1 <= topk <= nk (none is written when nq or nk is 0). nk is at most 32,768,
+ * batch x heads at most 65,535 and batch x heads x (nq + nk) below 2^22.
  * The workspace holds the means and scores: h3a_block_select_workspace_size
  * bytes, 256-byte aligned, free again once the call's work has run.
  */
@@ -167,7 +168,7 @@ H3A_API int h3a_block_select(const h3a_block_select_args *args, void *stream);
  * q, k, v, o and lse as for h3a_attn_fwd (dense, head_dim 128); block_index is
  * int32 with unit stride between a row's entries and index_stride (batch, head,
  * query block) between rows; count_stride likewise. max_blocks is at most
- * H3A_SPARSE_MAX_BLOCKS. A launch of few query blocks cuts the lists into
+ * H3A_SPARSE_MAX_BLOCKS, and batch x heads x query blocks below 2^20. A launch of few query blocks cuts the lists into
  * pieces, whose partial results (fp32) take a workspace of
  * h3a_attn_sparse_workspace_size bytes, 256-byte aligned; without one the lists
  * run whole. workspace NULL with workspace_bytes H3A_WORKSPACE_ASK: the call
