@@ -4,7 +4,8 @@
 //   O = softmax(scale * Q K_L^T) V_L,  LSE = log sum exp(scale * Q K_L^T)
 // over the keys of the listed blocks, each as often as it is named. Entries past
 // the row's count or outside the key blocks name nothing; a row without keys
-// has O = 0 and LSE = -inf.
+// has O = 0 and LSE = -inf. As in the dense forward the weights are rounded to
+// bf16 for the product with V, and nothing else before O (attn_tile.h).
 //
 // A listed block is one key tile of attn_tile (or two key blocks of attn_unit),
 // so the tile's pipeline runs as in the dense forward with the list in place of

@@ -26,6 +26,14 @@
 //     of two, exactly. A tile whose row sum passes 2^64 (a score more than
 //     ~64 log2 units above the offset, up to p = inf) is recomputed from K
 //     in global memory against its exact max.
+//   * P is rounded to bf16 for the PV product, by at most 2^-8 of each weight:
+//     an MFMA takes both operands in one type, and V is bf16. The row sum and the
+//     LSE take P in fp32, and O and the sum stay in fp32 up to the output's own
+//     rounding. Against 64 bits the output is off by 0.0022 to 0.0023 (in the
+//     norm; 1,024 to 9,984 keys a row), where rounding the exact result to bf16
+//     costs 0.0017 and rounding P alone 0.0015. P as a sum of two bf16 parts
+//     would remove the second for twice the PV MFMAs, half as many again in all,
+//     of a kernel that the matrix cores bound.
 // LDS rows are 256 bytes, unpadded; the 16-byte chunk c of row r is stored at
 // chunk c ^ swz(r), swz(r) = 4*(r & 3) + ((r >> 2) & 3). Both read patterns are
 // then bank-conflict free: the K reads (16 consecutive rows, one chunk) and the

@@ -104,7 +104,11 @@ def sparse_attn_func(
     (default: all; clamped to [0, n]). Entries may come in any order; a block
     named twice counts twice, as two keys would; entries outside [0, nk) name
     nothing. A row without keys has ``out`` 0 and ``lse`` -inf. Lists hold at most
-    7,168 entries.
+    7,168 entries. ``out`` and ``lse``, where given, overlap no input.
+
+    Scores, sums and ``lse`` are fp32; the softmax weights are rounded to bf16 for
+    the product with ``v`` (by at most 2^-8 of each), as in
+    :func:`flash_attn_func`, and the result once more.
     """
 
     q, k, v = _as_kernel_operand(q, "q"), _as_kernel_operand(k, "k"), _as_kernel_operand(v, "v")

@@ -165,14 +165,17 @@ H3A_API int h3a_block_select(const h3a_block_select_args *args, void *stream);
  *   O = softmax(scale * Q K_L^T) V_L,  LSE = log(sum(exp(scale * Q K_L^T)))
  * Entries may come in any order; one named twice counts twice, one outside
  * [0, nk) names nothing, and a row without keys gives O = 0 and LSE = -inf.
- * q, k, v, o and lse as for h3a_attn_fwd (dense, head_dim 128); block_index is
- * int32 with unit stride between a row's entries and index_stride (batch, head,
- * query block) between rows; count_stride likewise. max_blocks is at most
- * H3A_SPARSE_MAX_BLOCKS, and batch x heads x query blocks below 2^20. A launch of few query blocks cuts the lists into
- * pieces, whose partial results (fp32) take a workspace of
- * h3a_attn_sparse_workspace_size bytes, 256-byte aligned; without one the lists
- * run whole. workspace NULL with workspace_bytes H3A_WORKSPACE_ASK: the call
- * launches, or returns H3A_NEED_WORKSPACE without launching where it takes one.
+ * Scores, sums and LSE are fp32; the weights are rounded to bf16 for the product
+ * with V, as in h3a_attn_fwd, and the result once more.
+ * q, k, v, o and lse as for h3a_attn_fwd (dense, head_dim 128), o and lse apart
+ * from every input; block_index is int32 with unit stride between a row's entries
+ * and index_stride (batch, head, query block) between rows; count_stride likewise.
+ * max_blocks is at most H3A_SPARSE_MAX_BLOCKS, and batch x heads x query blocks
+ * below 2^20. A launch of few query blocks cuts the lists into pieces, whose
+ * partial results (fp32) take a workspace of h3a_attn_sparse_workspace_size
+ * bytes, 256-byte aligned; without one the lists run whole. workspace NULL with
+ * workspace_bytes H3A_WORKSPACE_ASK: the call launches, or returns
+ * H3A_NEED_WORKSPACE without launching where it takes one.
  */
 #define H3A_SPARSE_MAX_BLOCKS 7168
 
