@@ -300,7 +300,7 @@ struct LinearParams {
     int32_t m, k, n;       // k and n multiples of 8
     int32_t act, gated, bias_f32, gate_f32, index_i64;
     // Set by plan_linear: the tile shape (-1: the form for few tokens, -2: more
-    // tiles than a launch takes), its tiles
+    // work items than a launch takes), its tiles
     // over tokens and features, the token tiles of a group of their order, and
     // of the tiles past n_full the pieces along K, whose sums go to ws.
     int32_t shape, m_tiles, n_tiles, group_m, n_full, split;

@@ -435,22 +435,33 @@ hipError_t launch_rows_t(const LinearParams& p, int waves, hipStream_t stream) {
     return hipGetLastError();
 }
 
+// Blocks of rows per workgroup: x is read once for each of them, and a launch
+// wants a workgroup per CU (us, 1 / 2 / 4 blocks: 16 x 5,376 x 32,256 106 / 83
+// / 72; 16 x 5,376 x 14,336 gated - / 78 / 67; 32 x 5,376 x 5,376 36 / 23 / 34;
+// 4 x 14,336 x 5,376 46 / 42 / 74). Waves so that 16 per CU share a launch,
+// each with a chunk at least.
+struct RowsForm {
+    int na, waves;
+    int64_t groups;  // workgroups
+};
+
+RowsForm rows_form(const LinearParams& p, int cus) {
+    const int64_t blocks = (int64_t)((p.n + 15) / 16) * (p.gated ? 2 : 1);  // (the tokens are one block of 16 NB)
+    RowsForm f;
+    f.na = blocks >= 4ll * cus ? 4 : blocks >= cus || p.gated ? 2 : 1;
+    f.groups = (blocks + f.na - 1) / f.na;
+    f.waves = 4;
+    while (f.waves < (f.na == 1 ? 16 : 8) && f.groups * f.waves < 16ll * cus && f.waves * 128 < p.k * 2) f.waves *= 2;
+    return f;
+}
+
 template <int NB>
 hipError_t launch_rows(const LinearParams& p, int cus, hipStream_t stream) {
-    // Blocks of rows per workgroup: x is read once for each of them, and a launch
-    // wants a workgroup per CU (us, 1 / 2 / 4 blocks: 16 x 5,376 x 32,256 106 / 83
-    // / 72; 16 x 5,376 x 14,336 gated - / 78 / 67; 32 x 5,376 x 5,376 36 / 23 / 34;
-    // 4 x 14,336 x 5,376 46 / 42 / 74). Waves so that 16 per CU share a launch,
-    // each with a chunk at least.
-    const int64_t blocks = (int64_t)((p.n + 15) / 16) * (p.gated ? 2 : 1) * ((p.m + 16 * NB - 1) / (16 * NB));
-    const int na = blocks >= 4ll * cus ? 4 : blocks >= cus || p.gated ? 2 : 1;
-    const int64_t groups = (blocks + na - 1) / na;
-    int waves = 4;
-    while (waves < (na == 1 ? 16 : 8) && groups * waves < 16ll * cus && waves * 128 < p.k * 2) waves *= 2;
-    if (p.gated) return na == 4 ? launch_rows_t<4, NB, true>(p, waves, stream) : launch_rows_t<2, NB, true>(p, waves, stream);
-    return na == 4   ? launch_rows_t<4, NB, false>(p, waves, stream)
-           : na == 2 ? launch_rows_t<2, NB, false>(p, waves, stream)
-                     : launch_rows_t<1, NB, false>(p, waves, stream);
+    const RowsForm f = rows_form(p, cus);
+    if (p.gated) return f.na == 4 ? launch_rows_t<4, NB, true>(p, f.waves, stream) : launch_rows_t<2, NB, true>(p, f.waves, stream);
+    return f.na == 4   ? launch_rows_t<4, NB, false>(p, f.waves, stream)
+           : f.na == 2 ? launch_rows_t<2, NB, false>(p, f.waves, stream)
+                       : launch_rows_t<1, NB, false>(p, f.waves, stream);
 }
 
 }  // namespace
@@ -458,9 +469,12 @@ hipError_t launch_rows(const LinearParams& p, int cus, hipStream_t stream) {
 void plan_linear(LinearParams& p, int cus, int64_t* workspace) {
     if (cus <= 0) cus = 256;
     *workspace = 0;
-    p.shape = kRowsForm;
-    if (p.m <= kRowsMaxTokens) return;
     p.shape = kNoForm;
+    if (p.m <= kRowsMaxTokens) {
+        const RowsForm f = rows_form(p, cus);
+        if (f.groups * 64 * f.waves <= UINT32_MAX) p.shape = kRowsForm;  // work items of a launch
+        return;
+    }
     const int steps = (p.k + kPK - 1) / kPK;
     float best_us = 0.f;
     for (int i = 0; i < (int)(sizeof(kShapes) / sizeof(kShapes[0])); ++i) {

@@ -27,8 +27,9 @@ extern "C" {
  * x, weight, residual and y are bf16 with rows of unit column stride; bias and
  * gate bf16 or fp32; index int32 or int64. k and n are positive multiples of 8;
  * rows are 16-byte aligned (strides multiples of 8 elements; fp32 gate rows of
- * 4); 256 rows of x and of weight span less than 2^31 bytes. y may be the
- * residual, and must not overlap any other operand.
+ * 4); 256 rows of x and of weight span less than 2^31 bytes; a launch of 2^32
+ * work items or more is refused (for at most 32 rows of x: of some 2^30 rows of
+ * weight). y may be the residual, and must not overlap any other operand.
  * A launch whose last round of tiles would leave CUs idle cuts those tiles into
  * pieces along k, whose sums (fp32) take a workspace of
  * h3a_linear_workspace_size bytes, 256-byte aligned; without one every tile runs
