@@ -171,5 +171,7 @@ class BlockSparseKernel:
     ) -> tuple[torch.Tensor, torch.Tensor]:
         if causal:
             raise RuntimeError("H3 sparse HIP attention supports only non-causal attention")
-        topk = max(1, math.ceil(self.keep * _blocks(k.shape[1], BLOCK_K)))
+        # (Less 1e-9: the product may pass the whole number that is meant, as 0.07 *
+        # 100 does 7.)
+        topk = max(1, math.ceil((self.keep - 1e-9) * _blocks(k.shape[1], BLOCK_K)))
         return sparse_attn_func(q, k, v, select_key_blocks(q, k, topk, always=self.always), softmax_scale=softmax_scale)
