@@ -24,6 +24,25 @@ int check_index(const char* fn, const void* index, int32_t dtype, int64_t n_inde
     return H3A_OK;
 }
 
+// Rows of memory: `rows` of `bytes` each, `pitch` apart.
+struct RowSpan {
+    const void* ptr;
+    int64_t rows, bytes, pitch;
+};
+
+// Whether two sets of rows share a byte. At one pitch (a single row has any) they
+// may lie side by side, as columns of one buffer; at two, rows in a common range
+// count as shared.
+bool overlap(const RowSpan& a, const RowSpan& b) {
+    const int64_t d = (int64_t)((uintptr_t)b.ptr - (uintptr_t)a.ptr);
+    if (d >= (a.rows - 1) * a.pitch + a.bytes || -d >= (b.rows - 1) * b.pitch + b.bytes) return false;
+    if (a.rows == 1 && b.rows == 1) return true;
+    const int64_t pitch = a.rows == 1 ? b.pitch : a.pitch;
+    if (b.rows > 1 && b.pitch != pitch) return true;
+    const int64_t at = (d % pitch + pitch) % pitch;  // where b's rows start in a's
+    return at < a.bytes || at + b.bytes > pitch;
+}
+
 // A (batch, seq, head, 128) bf16 view of `rows` rows a head.
 int check_view(const char* fn, const char* name, const void* ptr, const int64_t* st, int64_t window) {
     if (!ptr || !aligned16(ptr)) return fail(H3A_EINVAL, "%s: %s must be a 16-byte aligned device pointer", fn, name);
@@ -233,6 +252,17 @@ int h3a_linear(const h3a_linear_args* a, void* stream) {
     bool empty = false;
     const int rc = prepare_linear(a, p, &need, &empty);
     if (rc != H3A_OK || empty) return rc;
+    // y apart from what other workgroups still read (it may be the residual, whose
+    // elements are read by the lanes that store them).
+    const int64_t w_rows = (p.gated ? 2 : 1) * (int64_t)p.n;
+    const RowSpan y{p.y, p.m, 2 * (int64_t)p.n, p.y_rs};
+    const RowSpan res{p.residual, p.m, 2 * (int64_t)p.n, p.res_rs};
+    const bool in_place = res.ptr == y.ptr && (p.m == 1 || res.pitch == y.pitch);
+    if (overlap(y, RowSpan{p.x, p.m, 2 * (int64_t)p.k, p.x_rs}) || overlap(y, RowSpan{p.w, w_rows, 2 * (int64_t)p.k, p.w_rs}) ||
+        (p.bias != nullptr && overlap(y, RowSpan{p.bias, 1, w_rows * (p.bias_f32 ? 4 : 2), 0})) ||
+        (p.gate != nullptr && overlap(y, RowSpan{p.gate, p.table_rows, (int64_t)p.n * (p.gate_f32 ? 4 : 2), p.gate_rs})) ||
+        (p.residual != nullptr && !in_place && overlap(y, res)))
+        return fail(H3A_EINVAL, "%s: y overlaps an operand (it may be the residual itself)", fn);
     if (need > 0) {
         if (a->workspace == nullptr && a->workspace_bytes == H3A_WORKSPACE_ASK) return H3A_NEED_WORKSPACE;
         if (a->workspace != nullptr && ((uintptr_t)a->workspace & 255u) == 0 && a->workspace_bytes >= need) {

@@ -59,7 +59,7 @@ def fused_linear(
     ``out``: (..., n) bf16. ``activation``: None, "silu", "gelu", "gelu_tanh" or
     "relu". With ``gated`` the weight (and bias) hold 2 n rows, values then gates,
     and the product is ``value * act(gate)``. ``k`` and ``n`` are multiples of 8.
-    ``out`` may be the residual itself.
+    ``out`` may be the residual itself and overlaps no other operand (ValueError).
     """
 
     if weight.dim() != 2 or weight.dtype != torch.bfloat16:
