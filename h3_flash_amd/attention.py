@@ -61,7 +61,11 @@ def _as_kernel_operand(t: torch.Tensor, name: str) -> torch.Tensor:
     if not t.is_cuda:
         raise RuntimeError(f"{name} must be on a ROCm device, got {t.device}")
     b, s, h, d = t.stride()
-    return t if d == 1 and not (b | s | h) & 7 and not t.data_ptr() & 15 else t.contiguous()
+    if d == 1 and not (b | s | h) & 7 and not t.data_ptr() & 15:
+        return t
+    # (contiguous() returns t itself where it is contiguous but starts anywhere, or
+    # has one token at an odd stride.)
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def flash_attn_func(
