@@ -561,7 +561,6 @@ rmsnorm_residual_gate_rmsnorm_modulate = Launch(
     "h3a_rmsnorm_residual_gate_rmsnorm_modulate", RmsnormResidualGateRmsnormModulateArgs
 )
 block_select = Launch("h3a_block_select", BlockSelectArgs)
-block_select_workspace_size = Launch("h3a_block_select_workspace_size", BlockSelectArgs, ctypes.c_int64, on_stream=False)
 attn_sparse = Launch("h3a_attn_sparse", AttnSparseArgs)
 attn_sparse_workspace_size = Launch("h3a_attn_sparse_workspace_size", AttnSparseArgs, ctypes.c_int64, on_stream=False)
 

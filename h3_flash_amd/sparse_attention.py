@@ -30,7 +30,8 @@ def _blocks(n: int, size: int) -> int:
 
 
 def _select_workspace(heads: int, nq: int, nk: int) -> int:
-    """h3a_block_select_workspace_size without the call: the means and scores."""
+    """What h3a_block_select_workspace_size returns, without the call: the means and
+    scores, each from a 256-byte boundary on (the tests hold the two equal)."""
 
     return sum(-(-heads * n // 256) * 256 for n in (nq * 512, nk * 512, nq * nk * 4))
 
