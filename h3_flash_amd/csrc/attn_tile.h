@@ -1292,9 +1292,10 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(AttnParams p) {
 #pragma unroll
     for (int c = 0; c < kMaxP; ++c) {
         if (c >= n) break;
-        // Every piece holds keys and writes its rows up to the last query row
-        // (waves past it write none, and none is read here); a -inf LSE would
-        // still weigh nothing.
+        // Every piece writes its rows up to the last query row (waves past it
+        // write none, and none is read here). A piece of a list may hold no block:
+        // zero rows and an LSE of -inf, which weigh nothing; where all pieces are
+        // such, the difference of two infinities would be NaN.
         const float w = lq[c] == -INFINITY ? 0.f : __expf(lq[c] - lse_max);
         wsum += w;
 #pragma unroll
