@@ -13,6 +13,7 @@ from .attention import (
     provenance,
 )
 from .context_parallel import chunked_attention, merge_attention
+from .fp8 import fused_linear_fp8, quantize_fp8, quantize_fp8_weight
 from .linear import fused_linear
 from .prologue import fused_qk_norm_rope, fused_qknorm_rope
 from .sparse_attention import BlockSparseKernel, select_key_blocks, sparse_attn_func
@@ -24,6 +25,7 @@ __all__ = [
     "flash_attn_func",
     "flash_attn_varlen_func",
     "fused_linear",
+    "fused_linear_fp8",
     "fused_qk_norm_rope",
     "fused_qknorm_rope",
     "hip_forward_op",
@@ -31,6 +33,8 @@ __all__ = [
     "load_kernel",
     "merge_attention",
     "provenance",
+    "quantize_fp8",
+    "quantize_fp8_weight",
     "select_key_blocks",
     "sparse_attn_func",
 ]

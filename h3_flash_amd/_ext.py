@@ -1,4 +1,4 @@
-"""ctypes binding of the C ABI in ``include/h3attn.h`` and ``include/h3block.h``.
+"""ctypes binding of the C ABI in ``include/h3attn.h``, ``include/h3block.h`` and ``include/h3fp8.h``.
 
 The structures below mirror the headers' argument structs field for field. Loading fails loudly (``RuntimeError``) when the library has
 not been built: there is no other implementation behind these entry points.
@@ -29,6 +29,7 @@ H3A_DTYPE_BF16 = 0
 H3A_DTYPE_F32 = 1
 H3A_DTYPE_I32 = 2
 H3A_DTYPE_I64 = 3
+H3A_DTYPE_F8E4M3 = 4
 
 # Bytes of the device array behind h3a_attn_fwd_noalloc (H3A_NOALLOC_SCRATCH_BYTES).
 H3A_NOALLOC_SCRATCH_BYTES = 64 << 20
@@ -399,6 +400,119 @@ class AttnSparseArgs(ctypes.Structure):
     ]
 
 
+class QuantizeFp8Args(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("x", ctypes.c_void_p),
+        ("x_dtype", ctypes.c_int32),
+        ("q", ctypes.c_void_p),
+        ("scale", ctypes.c_void_p),
+        ("rows", ctypes.c_int64),
+        ("cols", ctypes.c_int64),
+        ("block_rows", ctypes.c_int64),
+        ("parts", ctypes.c_int64),
+        ("x_stride", ctypes.c_int64),
+        ("q_stride", ctypes.c_int64),
+        ("scale_stride", ctypes.c_int64),
+    ]
+
+
+class RmsnormModulateFp8Args(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("x", ctypes.c_void_p),
+        ("q_out", ctypes.c_void_p),
+        ("scale_out", ctypes.c_void_p),
+        ("weight", ctypes.c_void_p),
+        ("w_dtype", ctypes.c_int32),
+        ("scale", ctypes.c_void_p),
+        ("shift", ctypes.c_void_p),
+        ("table_dtype", ctypes.c_int32),
+        ("scale_stride", ctypes.c_int64),
+        ("shift_stride", ctypes.c_int64),
+        ("table_rows", ctypes.c_int64),
+        ("index", ctypes.c_void_p),
+        ("index_dtype", ctypes.c_int32),
+        ("n_index", ctypes.c_int64),
+        ("rows", ctypes.c_int64),
+        ("cols", ctypes.c_int64),
+        ("x_stride", ctypes.c_int64),
+        ("q_stride", ctypes.c_int64),
+        ("scale_out_stride", ctypes.c_int64),
+        ("eps", ctypes.c_float),
+    ]
+
+
+class ResidualGateRmsnormModulateFp8Args(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("residual", ctypes.c_void_p),
+        ("branch", ctypes.c_void_p),
+        ("hidden_out", ctypes.c_void_p),
+        ("q_out", ctypes.c_void_p),
+        ("scale_out", ctypes.c_void_p),
+        ("weight", ctypes.c_void_p),
+        ("w_dtype", ctypes.c_int32),
+        ("gate", ctypes.c_void_p),
+        ("scale", ctypes.c_void_p),
+        ("shift", ctypes.c_void_p),
+        ("table_dtype", ctypes.c_int32),
+        ("gate_stride", ctypes.c_int64),
+        ("scale_stride", ctypes.c_int64),
+        ("shift_stride", ctypes.c_int64),
+        ("table_rows", ctypes.c_int64),
+        ("index", ctypes.c_void_p),
+        ("index_dtype", ctypes.c_int32),
+        ("n_index", ctypes.c_int64),
+        ("rows", ctypes.c_int64),
+        ("cols", ctypes.c_int64),
+        ("residual_stride", ctypes.c_int64),
+        ("branch_stride", ctypes.c_int64),
+        ("hidden_stride", ctypes.c_int64),
+        ("q_stride", ctypes.c_int64),
+        ("scale_out_stride", ctypes.c_int64),
+        ("eps", ctypes.c_float),
+    ]
+
+
+class LinearFp8Args(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("x", ctypes.c_void_p),
+        ("x_dtype", ctypes.c_int32),
+        ("x_scale", ctypes.c_void_p),
+        ("weight", ctypes.c_void_p),
+        ("weight_scale", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("bias_dtype", ctypes.c_int32),
+        ("residual", ctypes.c_void_p),
+        ("gate", ctypes.c_void_p),
+        ("gate_dtype", ctypes.c_int32),
+        ("gate_stride", ctypes.c_int64),
+        ("table_rows", ctypes.c_int64),
+        ("index", ctypes.c_void_p),
+        ("index_dtype", ctypes.c_int32),
+        ("n_index", ctypes.c_int64),
+        ("y", ctypes.c_void_p),
+        ("y_dtype", ctypes.c_int32),
+        ("y_scale", ctypes.c_void_p),
+        ("m", ctypes.c_int64),
+        ("k", ctypes.c_int64),
+        ("n", ctypes.c_int64),
+        ("x_stride", ctypes.c_int64),
+        ("x_scale_stride", ctypes.c_int64),
+        ("weight_stride", ctypes.c_int64),
+        ("weight_scale_stride", ctypes.c_int64),
+        ("residual_stride", ctypes.c_int64),
+        ("y_stride", ctypes.c_int64),
+        ("y_scale_stride", ctypes.c_int64),
+        ("activation", ctypes.c_int32),
+        ("gated", ctypes.c_int32),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+    ]
+
+
 # Every function the headers declare, with its ctypes signature.
 SIGNATURES = {
     "h3a_attn_fwd": (ctypes.c_int, [ctypes.POINTER(AttnArgs), ctypes.c_void_p]),
@@ -426,6 +540,15 @@ SIGNATURES = {
     "h3a_block_select_workspace_size": (ctypes.c_int64, [ctypes.POINTER(BlockSelectArgs)]),
     "h3a_attn_sparse": (ctypes.c_int, [ctypes.POINTER(AttnSparseArgs), ctypes.c_void_p]),
     "h3a_attn_sparse_workspace_size": (ctypes.c_int64, [ctypes.POINTER(AttnSparseArgs)]),
+    "h3a_quantize_fp8": (ctypes.c_int, [ctypes.POINTER(QuantizeFp8Args), ctypes.c_void_p]),
+    "h3a_rmsnorm_modulate_fp8": (ctypes.c_int, [ctypes.POINTER(RmsnormModulateFp8Args), ctypes.c_void_p]),
+    "h3a_residual_gate_rmsnorm_modulate_fp8": (
+        ctypes.c_int,
+        [ctypes.POINTER(ResidualGateRmsnormModulateFp8Args), ctypes.c_void_p],
+    ),
+    "h3a_linear_fp8": (ctypes.c_int, [ctypes.POINTER(LinearFp8Args), ctypes.c_void_p]),
+    "h3a_linear_fp8_workspace_size": (ctypes.c_int64, [ctypes.POINTER(LinearFp8Args)]),
+    "h3a_linear_fp8_required_workspace": (ctypes.c_int64, [ctypes.POINTER(LinearFp8Args)]),
     "h3a_clock_sample": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
     "h3a_last_error": (ctypes.c_char_p, []),
     "h3a_abi_version": (ctypes.c_int, []),
@@ -563,6 +686,12 @@ rmsnorm_residual_gate_rmsnorm_modulate = Launch(
 block_select = Launch("h3a_block_select", BlockSelectArgs)
 attn_sparse = Launch("h3a_attn_sparse", AttnSparseArgs)
 attn_sparse_workspace_size = Launch("h3a_attn_sparse_workspace_size", AttnSparseArgs, ctypes.c_int64, on_stream=False)
+
+quantize_fp8 = Launch("h3a_quantize_fp8", QuantizeFp8Args)
+rmsnorm_modulate_fp8 = Launch("h3a_rmsnorm_modulate_fp8", RmsnormModulateFp8Args)
+residual_gate_rmsnorm_modulate_fp8 = Launch("h3a_residual_gate_rmsnorm_modulate_fp8", ResidualGateRmsnormModulateFp8Args)
+linear_fp8 = Launch("h3a_linear_fp8", LinearFp8Args)
+linear_fp8_workspace_size = Launch("h3a_linear_fp8_workspace_size", LinearFp8Args, ctypes.c_int64, on_stream=False)
 
 
 def provenance() -> dict:

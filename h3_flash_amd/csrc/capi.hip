@@ -10,6 +10,7 @@
 
 #include "capi_util.h"
 #include "h3attn.h"
+#include "h3fp8.h"
 #include "kernels.h"
 
 namespace {
@@ -412,6 +413,25 @@ int check_rows(const char* fn, const char* name, const void* ptr, int64_t stride
     return H3A_OK;
 }
 
+// A norm's result in 8 bits; its rows are the vector path's alone.
+int check_modulate_fp8(const char* fn, void* q, int64_t q_stride, void* scale, int64_t scale_stride, bool vec, h3a::ModulateParams& p) {
+    if (p.cols % 16 != 0 || p.cols > H3A_NORM_FP8_MAX_COLS)
+        return fail(H3A_EUNSUPPORTED, "%s: cols must be a multiple of 16, at most %d, got %d", fn, H3A_NORM_FP8_MAX_COLS, p.cols);
+    // (A workgroup of 256 per row: 2^32 work items a launch.)
+    if (p.rows >= ((int64_t)1 << 24)) return fail(H3A_EUNSUPPORTED, "%s: extents too large", fn);
+    if (p.rows == 0) return H3A_OK;
+    if (!vec) return fail(H3A_EINVAL, "%s: rows, weight and tables must be 16-byte aligned", fn);
+    if (!q || !aligned16(q) || q_stride < p.cols || q_stride % 16)
+        return fail(H3A_EINVAL, "%s: q_out must have 16-byte aligned rows of at least cols bytes", fn);
+    if (!scale || !aligned16(scale) || scale_stride < (p.cols + 127) / 128 || scale_stride % 16)
+        return fail(H3A_EINVAL, "%s: scale_out's rows must start at multiples of 16 bytes and hold %d", fn, (p.cols + 127) / 128);
+    p.q = q;
+    p.q_scale = (uint8_t*)scale;
+    p.q_stride = q_stride;
+    p.q_scale_stride = scale_stride;
+    return H3A_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -776,6 +796,57 @@ int h3a_residual_gate_rmsnorm_modulate(const h3a_residual_gate_rmsnorm_modulate_
     p.out_stride = a->normed_stride; p.hidden_stride = a->hidden_stride;
     p.gate_stride = a->gate_stride; p.scale_stride = a->scale_stride; p.shift_stride = a->shift_stride;
     hipError_t e = h3a::launch_modulate(p, vec, (hipStream_t)stream);
+    if (e != hipSuccess) return fail(H3A_ELAUNCH, "%s: launch failed: %s", fn, hipGetErrorString(e));
+    return H3A_OK;
+}
+
+int h3a_rmsnorm_modulate_fp8(const h3a_rmsnorm_modulate_fp8_args* a, void* stream) {
+    g_err[0] = '\0';
+    const char* fn = "h3a_rmsnorm_modulate_fp8";
+    if (a == nullptr) return fail(H3A_EINVAL, "%s: args is NULL", fn);
+    if (a->abi_version != H3A_ABI_VERSION)
+        return fail(H3A_EINVAL, "%s: abi_version %d, library is %d", fn, a->abi_version, H3A_ABI_VERSION);
+    h3a::ModulateParams p{};
+    bool vec = false;
+    const void* tables[2] = {a->scale, a->shift};
+    const int64_t strides[2] = {a->scale_stride, a->shift_stride};
+    int rc = prepare_modulate(fn, a->weight, a->w_dtype, tables, strides, 2, a->table_dtype, a->table_rows, a->index,
+                              a->index_dtype, a->n_index, a->rows, a->cols, a->eps, p, &vec);
+    if (rc != H3A_OK) return rc;
+    if ((rc = check_rows(fn, "x", a->x, a->x_stride, a->rows, a->cols, &vec)) != H3A_OK) return rc;
+    if ((rc = check_modulate_fp8(fn, a->q_out, a->q_stride, a->scale_out, a->scale_out_stride, vec, p)) != H3A_OK) return rc;
+    if (a->rows == 0) return H3A_OK;
+    p.x = a->x; p.scale = a->scale; p.shift = a->shift;
+    p.x_stride = a->x_stride;
+    p.scale_stride = a->scale_stride; p.shift_stride = a->shift_stride;
+    hipError_t e = h3a::launch_modulate_fp8(p, (hipStream_t)stream);
+    if (e != hipSuccess) return fail(H3A_ELAUNCH, "%s: launch failed: %s", fn, hipGetErrorString(e));
+    return H3A_OK;
+}
+
+int h3a_residual_gate_rmsnorm_modulate_fp8(const h3a_residual_gate_rmsnorm_modulate_fp8_args* a, void* stream) {
+    g_err[0] = '\0';
+    const char* fn = "h3a_residual_gate_rmsnorm_modulate_fp8";
+    if (a == nullptr) return fail(H3A_EINVAL, "%s: args is NULL", fn);
+    if (a->abi_version != H3A_ABI_VERSION)
+        return fail(H3A_EINVAL, "%s: abi_version %d, library is %d", fn, a->abi_version, H3A_ABI_VERSION);
+    h3a::ModulateParams p{};
+    bool vec = false;
+    const void* tables[3] = {a->gate, a->scale, a->shift};
+    const int64_t strides[3] = {a->gate_stride, a->scale_stride, a->shift_stride};
+    int rc = prepare_modulate(fn, a->weight, a->w_dtype, tables, strides, 3, a->table_dtype, a->table_rows, a->index,
+                              a->index_dtype, a->n_index, a->rows, a->cols, a->eps, p, &vec);
+    if (rc != H3A_OK) return rc;
+    if ((rc = check_rows(fn, "residual", a->residual, a->residual_stride, a->rows, a->cols, &vec)) != H3A_OK) return rc;
+    if ((rc = check_rows(fn, "branch", a->branch, a->branch_stride, a->rows, a->cols, &vec)) != H3A_OK) return rc;
+    if ((rc = check_rows(fn, "hidden_out", a->hidden_out, a->hidden_stride, a->rows, a->cols, &vec)) != H3A_OK) return rc;
+    if ((rc = check_modulate_fp8(fn, a->q_out, a->q_stride, a->scale_out, a->scale_out_stride, vec, p)) != H3A_OK) return rc;
+    if (a->rows == 0) return H3A_OK;
+    p.x = a->branch; p.residual = a->residual; p.hidden = a->hidden_out;
+    p.gate = a->gate; p.scale = a->scale; p.shift = a->shift;
+    p.x_stride = a->branch_stride; p.residual_stride = a->residual_stride; p.hidden_stride = a->hidden_stride;
+    p.gate_stride = a->gate_stride; p.scale_stride = a->scale_stride; p.shift_stride = a->shift_stride;
+    hipError_t e = h3a::launch_modulate_fp8(p, (hipStream_t)stream);
     if (e != hipSuccess) return fail(H3A_ELAUNCH, "%s: launch failed: %s", fn, hipGetErrorString(e));
     return H3A_OK;
 }

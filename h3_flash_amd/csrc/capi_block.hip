@@ -2,46 +2,10 @@
 // launch, as capi.hip does for h3attn.h.
 #include <math.h>
 
-#include "capi_util.h"
+#include "capi_linear.h"
 #include "h3block.h"
-#include "kernels.h"
 
 namespace {
-
-using h3a::aligned16;
-using h3a::aligned4;
-using h3a::fail;
-
-constexpr int64_t kMaxSpan = (int64_t)1 << 31;  // buffer offsets are 32-bit
-
-bool bf16_or_f32(int32_t dtype) { return dtype == H3A_DTYPE_BF16 || dtype == H3A_DTYPE_F32; }
-
-// The index that picks a modulation-table row per token.
-int check_index(const char* fn, const void* index, int32_t dtype, int64_t n_index, int64_t table_rows) {
-    if (!index || n_index <= 0 || table_rows <= 0) return fail(H3A_EINVAL, "%s: a table needs rows and an index of at least one entry", fn);
-    if (dtype != H3A_DTYPE_I32 && dtype != H3A_DTYPE_I64) return fail(H3A_EINVAL, "%s: unknown index dtype %d", fn, dtype);
-    if (((uintptr_t)index & (dtype == H3A_DTYPE_I64 ? 7u : 3u)) != 0) return fail(H3A_EINVAL, "%s: index is not aligned to its type", fn);
-    return H3A_OK;
-}
-
-// Rows of memory: `rows` of `bytes` each, `pitch` apart.
-struct RowSpan {
-    const void* ptr;
-    int64_t rows, bytes, pitch;
-};
-
-// Whether two sets of rows share a byte. At one pitch (a single row has any) they
-// may lie side by side, as columns of one buffer; at two, rows in a common range
-// count as shared.
-bool overlap(const RowSpan& a, const RowSpan& b) {
-    const int64_t d = (int64_t)((uintptr_t)b.ptr - (uintptr_t)a.ptr);
-    if (d >= (a.rows - 1) * a.pitch + a.bytes || -d >= (b.rows - 1) * b.pitch + b.bytes) return false;
-    if (a.rows == 1 && b.rows == 1) return true;
-    const int64_t pitch = a.rows == 1 ? b.pitch : a.pitch;
-    if (b.rows > 1 && b.pitch != pitch) return true;
-    const int64_t at = (d % pitch + pitch) % pitch;  // where b's rows start in a's
-    return at < a.bytes || at + b.bytes > pitch;
-}
 
 // A (batch, seq, head, 128) bf16 view of `rows` rows a head.
 int check_view(const char* fn, const char* name, const void* ptr, const int64_t* st, int64_t window) {
@@ -193,35 +157,8 @@ int prepare_linear(const h3a_linear_args* a, h3a::LinearParams& p, int64_t* need
     const int64_t rows = h3a::linear_max_tile();
     if (a->x_stride > (kMaxSpan - 1) / (2 * rows) || a->weight_stride > (kMaxSpan - 1) / (2 * rows))
         return fail(H3A_EUNSUPPORTED, "%s: %lld rows of x and of weight must span less than 2^31 bytes", fn, (long long)rows);
-    if (a->bias != nullptr) {
-        if (!bf16_or_f32(a->bias_dtype)) return fail(H3A_EINVAL, "%s: unknown bias dtype %d", fn, a->bias_dtype);
-        if (!aligned16(a->bias)) return fail(H3A_EINVAL, "%s: bias must be 16-byte aligned", fn);
-        p.bias = a->bias;
-        p.bias_f32 = a->bias_dtype == H3A_DTYPE_F32;
-    }
-    if (a->residual != nullptr) {
-        if (!aligned16(a->residual)) return fail(H3A_EINVAL, "%s: residual must be 16-byte aligned", fn);
-        if (a->residual_stride < a->n || a->residual_stride % 8)
-            return fail(H3A_EINVAL, "%s: residual_stride must be a multiple of 8 elements covering the row", fn);
-        p.residual = a->residual;
-        p.res_rs = a->residual_stride * 2;
-    }
-    if (a->gate != nullptr) {
-        if (!bf16_or_f32(a->gate_dtype)) return fail(H3A_EINVAL, "%s: unknown gate dtype %d", fn, a->gate_dtype);
-        if (!aligned16(a->gate)) return fail(H3A_EINVAL, "%s: gate must be 16-byte aligned", fn);
-        const int64_t size = a->gate_dtype == H3A_DTYPE_F32 ? 4 : 2;
-        if (a->gate_stride < a->n || a->gate_stride * size % 16)
-            return fail(H3A_EINVAL, "%s: gate rows must be 16-byte aligned and cover n", fn);
-        const int rc = check_index(fn, a->index, a->index_dtype, a->n_index, a->table_rows);
-        if (rc != H3A_OK) return rc;
-        p.gate = a->gate;
-        p.gate_f32 = size == 4;
-        p.gate_rs = a->gate_stride * size;
-        p.table_rows = a->table_rows;
-        p.index = a->index;
-        p.index_i64 = a->index_dtype == H3A_DTYPE_I64;
-        p.n_index = a->n_index;
-    }
+    const int rc = check_epilogue(fn, *a, p);
+    if (rc != H3A_OK) return rc;
     p.x = a->x; p.w = a->weight; p.y = a->y;
     p.x_rs = a->x_stride * 2; p.w_rs = a->weight_stride * 2; p.y_rs = a->y_stride * 2;
     p.m = (int32_t)a->m; p.k = (int32_t)a->k; p.n = (int32_t)a->n;
@@ -254,14 +191,9 @@ int h3a_linear(const h3a_linear_args* a, void* stream) {
     if (rc != H3A_OK || empty) return rc;
     // y apart from what other workgroups still read (it may be the residual, whose
     // elements are read by the lanes that store them).
-    const int64_t w_rows = (p.gated ? 2 : 1) * (int64_t)p.n;
     const RowSpan y{p.y, p.m, 2 * (int64_t)p.n, p.y_rs};
-    const RowSpan res{p.residual, p.m, 2 * (int64_t)p.n, p.res_rs};
-    const bool in_place = res.ptr == y.ptr && (p.m == 1 || res.pitch == y.pitch);
-    if (overlap(y, RowSpan{p.x, p.m, 2 * (int64_t)p.k, p.x_rs}) || overlap(y, RowSpan{p.w, w_rows, 2 * (int64_t)p.k, p.w_rs}) ||
-        (p.bias != nullptr && overlap(y, RowSpan{p.bias, 1, w_rows * (p.bias_f32 ? 4 : 2), 0})) ||
-        (p.gate != nullptr && overlap(y, RowSpan{p.gate, p.table_rows, (int64_t)p.n * (p.gate_f32 ? 4 : 2), p.gate_rs})) ||
-        (p.residual != nullptr && !in_place && overlap(y, res)))
+    if (overlap(y, RowSpan{p.x, p.m, 2 * (int64_t)p.k, p.x_rs}) ||
+        overlap(y, RowSpan{p.w, (p.gated ? 2 : 1) * (int64_t)p.n, 2 * (int64_t)p.k, p.w_rs}) || overlaps_epilogue(y, p, true))
         return fail(H3A_EINVAL, "%s: y overlaps an operand (it may be the residual itself)", fn);
     if (need > 0) {
         if (a->workspace == nullptr && a->workspace_bytes == H3A_WORKSPACE_ASK) return H3A_NEED_WORKSPACE;

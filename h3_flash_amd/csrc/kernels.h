@@ -217,10 +217,16 @@ struct ModulateParams {
     int32_t cols;
     int32_t w_f32, table_f32, index_i64;
     float eps;
+    // launch_modulate_fp8: the normed rows in 8 bits, in place of out (bytes)
+    void* q;
+    uint8_t* q_scale;
+    int64_t q_stride, q_scale_stride;
 };
 // Widest row the register-resident vector path takes.
 int modulate_max_vector_cols();
 hipError_t launch_modulate(const ModulateParams& p, bool vec, hipStream_t stream);
+// The vector path with its result in 8 bits; rows as it takes them.
+hipError_t launch_modulate_fp8(const ModulateParams& p, hipStream_t stream);
 
 struct SwigluParams {
     const void* x;
@@ -310,6 +316,33 @@ int linear_max_tile();  // rows of an operand that one buffer resource spans at 
 // Chooses the form; *workspace: the bytes that its pieces take (0: none).
 void plan_linear(LinearParams& p, int cus, int64_t* workspace);
 hipError_t launch_linear(const LinearParams& p, int cus, hipStream_t stream);
+
+// Rows, or blocks of 128 x 128 of a weight, to 8 bits. Byte strides.
+struct QuantizeParams {
+    const void* x;   // bf16 or fp32 (rows, cols), cols a multiple of 16, 16-byte rows
+    void* q;         // e4m3 (rows, cols)
+    uint8_t* scale;  // e8m0 (rows, or parts x ceil(part_rows / 128) blocks; ceil(cols / 128))
+    int64_t x_rs, q_rs, scale_rs;
+    int64_t rows, part_rows;  // blocks start anew after every part_rows rows
+    int32_t cols, x_f32, blocks;
+};
+hipError_t launch_quantize(const QuantizeParams& p, hipStream_t stream);
+
+// The matrix product of 8-bit operands with LinearParams' epilogue; its w, x and y
+// are e4m3 (x: or bf16, rounded to 8 bits first; y: or bf16), all strides in bytes.
+struct LinearFp8Params : LinearParams {
+    const uint8_t* x_scale;  // e8m0 (m, ceil(k / 128)), NULL: x is bf16
+    const uint8_t* w_scale;  // e8m0 (w_blocks or, gated, 2 w_blocks; ceil(k / 128))
+    int64_t x_scale_rs, w_scale_rs;
+    int32_t w_blocks;        // ceil(n / 128)
+    uint8_t* y_scale;        // e8m0 (m, ceil(n / 128)), NULL: y is bf16
+    int64_t y_scale_rs;
+    float* y32;              // set by the launcher: the unrounded result, for its quantisation
+};
+// Chooses the form; *workspace: the bytes that it takes, *required: those that it
+// cannot do without (the others are the sums of tiles in pieces).
+void plan_linear_fp8(LinearFp8Params& p, int cus, int64_t* required, int64_t* workspace);
+hipError_t launch_linear_fp8(const LinearFp8Params& p, int cus, hipStream_t stream);
 
 // Norm of a branch, gate, scaled residual, norm and modulation. Strides in elements.
 struct SandwichParams {

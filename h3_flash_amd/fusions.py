@@ -9,7 +9,9 @@ wrappers (src/h3_flash/runtime/kernels/fusions.py):
 * :func:`fused_qknorm_rope` (fusions.py:268-293), from :mod:`h3_flash_amd.prologue`
 
 and, for blocks that also normalise what a branch returns,
-:func:`fused_rmsnorm_residual_gate_rmsnorm_modulate`, which the reference lacks.
+:func:`fused_rmsnorm_residual_gate_rmsnorm_modulate`, which the reference lacks,
+and, with their result in 8 bits for :func:`h3_flash_amd.fused_linear_fp8`,
+:func:`fused_rmsnorm_modulate_fp8` and :func:`fused_residual_gate_rmsnorm_modulate_fp8`.
 
 Activations are bf16 (the dtype the H3 block runs in); weights and
 modulation tables may be bf16 or fp32, table indices int32 or int64. Table
@@ -27,7 +29,9 @@ from .prologue import fused_qknorm_rope
 __all__ = [
     "fused_qknorm_rope",
     "fused_residual_gate_rmsnorm_modulate",
+    "fused_residual_gate_rmsnorm_modulate_fp8",
     "fused_rmsnorm_modulate",
+    "fused_rmsnorm_modulate_fp8",
     "fused_rmsnorm_residual_gate_rmsnorm_modulate",
     "fused_swiglu",
 ]
@@ -84,6 +88,35 @@ def _tables(tables: list[torch.Tensor], columns: int, device: torch.device) -> l
         if column != 1 or row < columns:
             out[i] = t.contiguous()
     return out
+
+
+def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
+    """Rows of 16-byte chunks, as the launch reads them (else a copy)."""
+
+    row, column = t.stride()
+    if column == 1 and row * t.element_size() % 16 == 0 and row >= t.shape[1] and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _fp8_scales(lead: tuple[int, ...], columns: int, device: torch.device) -> tuple[torch.Tensor, int]:
+    """An empty (*lead, ceil(columns / 128)) tensor of e8m0 scales whose rows start at
+    multiples of 16 bytes, and their stride."""
+
+    groups = (columns + 127) // 128
+    pitch = (groups + 15) // 16 * 16
+    scale = torch.empty((*lead, pitch), dtype=torch.float8_e8m0fnu, device=device)
+    return (scale if pitch == groups else scale[..., :groups]), pitch
+
+
+def _norm_operand(x: torch.Tensor, name: str, columns: int) -> tuple[torch.Tensor, int, int]:
+    """:func:`_row_span`, of 16-byte aligned rows."""
+
+    held, rows, stride = _row_span(x, name, columns)
+    if stride % 8 or stride < columns or held.data_ptr() % 16:
+        held = _aligned_rows(_rows(held, name, columns))
+        stride = held.stride(0)
+    return held, rows, stride
 
 
 def _index(index: torch.Tensor, device: torch.device) -> torch.Tensor:
@@ -205,6 +238,65 @@ def fused_rmsnorm_residual_gate_rmsnorm_modulate(
             stride_r, stride_b, columns, columns, float(residual_scale), float(eps),
         )
     return hidden, normed
+
+
+def _norm_fp8_args(weight, tables, index, columns, device):
+    """The norm weight, the modulation tables in 16-byte aligned rows, and the index."""
+
+    if columns == 0 or columns % 16:
+        raise ValueError(f"the last dimension must be a positive multiple of 16, got {columns}")
+    weight = _vector(weight, columns, device, "weight")
+    weight = weight if weight.data_ptr() % 16 == 0 else weight.clone()
+    tables = [_aligned_rows(t) for t in _tables(tables, columns, device)]
+    return weight, tables, _index(index, device)
+
+
+def fused_rmsnorm_modulate_fp8(x, weight, scale, shift, index, eps):
+    """:func:`fused_rmsnorm_modulate` with its result in 8 bits, rounded from fp32:
+    returns ``(q, q_scale)`` as :func:`h3_flash_amd.quantize_fp8` does, for
+    :func:`h3_flash_amd.fused_linear_fp8`. The last dimension is a multiple of 16, at
+    most 16,384."""
+
+    columns = x.shape[-1]
+    device = x.device
+    held, rows, stride = _norm_operand(x, "x", columns)
+    weight, tables, index = _norm_fp8_args(weight, [scale, shift], index, columns, device)
+    scale, shift = tables
+    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=device)
+    q_scale, pitch = _fp8_scales(x.shape[:-1], columns, device)
+    _ext.rmsnorm_modulate_fp8.run(
+        device, _ext.ABI_VERSION, held.data_ptr(), q.data_ptr(), q_scale.data_ptr(), weight.data_ptr(), _dtype(weight),
+        scale.data_ptr(), shift.data_ptr(), _dtype(scale), scale.stride(0), shift.stride(0),
+        min(scale.shape[0], shift.shape[0]), *_index_args(index), rows, columns, stride, columns, pitch, float(eps),
+    )
+    return q, q_scale
+
+
+def fused_residual_gate_rmsnorm_modulate_fp8(residual, branch, gate, weight, scale, shift, index, eps):
+    """:func:`fused_residual_gate_rmsnorm_modulate` with its normed rows in 8 bits:
+    returns ``(hidden, q, q_scale)``, ``hidden`` in bf16, the others as from
+    :func:`fused_rmsnorm_modulate_fp8`."""
+
+    columns = residual.shape[-1]
+    device = residual.device
+    if branch.shape != residual.shape:
+        raise ValueError(f"residual {tuple(residual.shape)} and branch {tuple(branch.shape)} differ")
+    rows_r, rows, stride_r = _norm_operand(residual, "residual", columns)
+    rows_b, _, stride_b = _norm_operand(branch, "branch", columns)
+    if branch.device != device:
+        raise ValueError(f"residual and branch must be on one device, got {device} and {branch.device}")
+    weight, tables, index = _norm_fp8_args(weight, [gate, scale, shift], index, columns, device)
+    gate, scale, shift = tables
+    hidden = torch.empty(residual.shape, dtype=torch.bfloat16, device=device)
+    q = torch.empty(residual.shape, dtype=torch.float8_e4m3fn, device=device)
+    q_scale, pitch = _fp8_scales(residual.shape[:-1], columns, device)
+    _ext.residual_gate_rmsnorm_modulate_fp8.run(
+        device, _ext.ABI_VERSION, rows_r.data_ptr(), rows_b.data_ptr(), hidden.data_ptr(), q.data_ptr(), q_scale.data_ptr(),
+        weight.data_ptr(), _dtype(weight), gate.data_ptr(), scale.data_ptr(), shift.data_ptr(), _dtype(gate), gate.stride(0),
+        scale.stride(0), shift.stride(0), min(gate.shape[0], scale.shape[0], shift.shape[0]), *_index_args(index), rows, columns,
+        stride_r, stride_b, columns, columns, pitch, float(eps),
+    )
+    return hidden, q, q_scale
 
 
 def fused_swiglu(x):

@@ -15,18 +15,9 @@ from __future__ import annotations
 import torch
 
 from . import _ext
-from .fusions import _dtype, _index, _index_args, _row_span, _rows, _tables, _vector
+from .fusions import _aligned_rows, _dtype, _index, _index_args, _row_span, _rows, _tables, _vector
 
 __all__ = ["fused_linear"]
-
-
-def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
-    """Rows of 16-byte chunks, as the launch reads them (else a copy)."""
-
-    row, column = t.stride()
-    if column == 1 and row * t.element_size() % 16 == 0 and row >= t.shape[1] and t.data_ptr() % 16 == 0:
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _operand(x: torch.Tensor, name: str, columns: int) -> tuple[torch.Tensor, int, int]:

@@ -32,18 +32,19 @@ def activation_reference(z: torch.Tensor, kind: str | None) -> torch.Tensor:
     return z * torch.sigmoid(2.0 * math.sqrt(2.0 / math.pi) * (z + 0.044715 * z**3))
 
 
-def linear_reference(x, weight, bias=None, activation=None, gated=False, residual=None, gate=None, index=None):
+def linear_reference(x, weight, bias=None, activation=None, gated=False, residual=None, gate=None, index=None, *, sums=0.0, rounded=True):
     """``(y, bound)``. The bound: k products summed in any order in fp32 are off by
-    at most (k + 2) U times the sum of their magnitudes; the activations' slopes
-    are under 1.2, and they are evaluated to 2e-5 of their value; then the steps
-    of the epilogue and the rounding to bf16."""
+    at most (k + 2) U times the sum of their magnitudes (``sums`` more, relative to
+    it, where the products' sums are narrower); the activations' slopes are under
+    1.2, and they are evaluated to 2e-5 of their value; then the steps of the
+    epilogue and, unless ``rounded`` is false, the rounding to bf16."""
 
     x, w = x.double().reshape(-1, x.shape[-1]), weight.double()
     z = x @ w.t()
     size = x.abs() @ w.abs().t()
     if bias is not None:
         z, size = z + bias.double(), size + bias.double().abs()
-    off = (x.shape[1] + 2) * U * size
+    off = ((x.shape[1] + 2) * U + sums) * size
     if gated:
         (v, g), (ov, og) = z.chunk(2, -1), off.chunk(2, -1)
         a = activation_reference(g, activation)
@@ -58,7 +59,7 @@ def linear_reference(x, weight, bias=None, activation=None, gated=False, residua
     if residual is not None:
         r = residual.double().reshape(y.shape)
         y, off = y + r, off + 4 * U * (y.abs() + r.abs())
-    return y, off + 8 * U * y.abs() + H * (y.abs() + off) + 1e-37
+    return y, off + 8 * U * y.abs() + (H * (y.abs() + off) if rounded else 0.0) + 1e-37
 
 
 def _rms(x, eps):
