@@ -56,6 +56,8 @@ int prepare_linear_fp8(const h3a_linear_fp8_args* a, h3a::LinearFp8Params& p, in
         return fail(H3A_EINVAL, "%s: y must have 16-byte aligned rows of at least n elements", fn);
     }
     const int64_t rows = h3a::linear_max_tile(), x_size = x8 ? 1 : 2;
+    if (a->weight_scale_stride >= kMaxSpan / (2 * groups_of(a->n)))
+        return fail(H3A_EUNSUPPORTED, "%s: the scales of weight must span less than 2^31 bytes", fn);
     if (a->x_stride > (kMaxSpan - 1) / (x_size * rows) || a->weight_stride > (kMaxSpan - 1) / rows ||
         (x8 && a->x_scale_stride > (kMaxSpan - 1) / rows))
         return fail(H3A_EUNSUPPORTED, "%s: %lld rows of x and of weight must span less than 2^31 bytes", fn, (long long)rows);

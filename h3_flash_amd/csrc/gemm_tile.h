@@ -121,6 +121,30 @@ struct GemmRows {
 // the same for every load; i and the K step go into the scalar offset.
 __device__ __forceinline__ int gemm_chunk(int wave, int lane) { return ((lane & 7) ^ (4 * (wave & 1) + (lane >> 4))) << 4; }
 
+// Load j of this wave's share of a K step's rows (32 j rows on from the
+// wave's first), into LDS at dst + 4096 j. buffer_load ... lds writes 16
+// bytes per lane to LDS address M0 + 16*lane; M0 needs one wait state
+// before the load reads it. The row offsets stay in scalar registers and
+// the resources' bases move along K: three instructions a load, which fit
+// between two MFMAs (offsets formed per load took six, and held up the
+// lone wave's MFMAs).
+__device__ __forceinline__ void gemm_dma(const i32x4& rsrc, uint32_t voff, uint32_t soff, uint32_t dst, int j) {
+    asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, %4 offen lds"
+                 :
+                 : "s"(dst), "i"(j * 4096), "v"(voff), "s"(rsrc), "s"(soff)
+                 : "memory", "scc");
+}
+
+// The resource one K step further along its rows. The records stay: a
+// lane's offset in its row is under 128 bytes and a row is at least the
+// reduction long, so the row after the last one is out of range at every
+// base.
+__device__ __forceinline__ void gemm_advance(i32x4& r) {
+    const uint64_t base = ((uint64_t)(uint32_t)r.y << 32 | (uint32_t)r.x) + kPRow;
+    r.x = (int)(uint32_t)base;
+    r.y = (int)((uint32_t)(base >> 32) & 0xffffu);
+}
+
 // acc = W X^T over nk K steps; all waves of the workgroup call it. On return no
 // load is in flight and no wave reads the stages any more. kTailK: the last K
 // step is partial.
@@ -132,19 +156,6 @@ __device__ __forceinline__ void gemm_k_loop(const GemmRows& w_rows, const GemmRo
     const uint32_t dw = w_rows.lane, dx = x_rows.lane;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(const lds_char*)smem;
     const uint32_t lds_wave = lds0 + (uint32_t)wave * 1024u;
-    // Load j of this wave's share of a K step's rows (32 j rows on from the
-    // wave's first), into LDS at dst + 4096 j. buffer_load ... lds writes 16
-    // bytes per lane to LDS address M0 + 16*lane; M0 needs one wait state
-    // before the load reads it. The row offsets stay in scalar registers and
-    // the resources' bases move along K: three instructions a load, which fit
-    // between two MFMAs (offsets formed per load took six, and held up the
-    // lone wave's MFMAs).
-    auto dma1 = [&](const i32x4& rsrc, uint32_t voff, uint32_t soff, uint32_t dst, int j) __attribute__((always_inline)) {
-        asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, %4 offen lds"
-                     :
-                     : "s"(dst), "i"(j * 4096), "v"(voff), "s"(rsrc), "s"(soff)
-                     : "memory", "scc");
-    };
     uint32_t sow[T::kLoadsW], sox[T::kLoadsX];
 #pragma unroll
     for (int j = 0; j < T::kLoadsW; ++j) sow[j] = (uint32_t)j * w_rows.step;
@@ -152,19 +163,10 @@ __device__ __forceinline__ void gemm_k_loop(const GemmRows& w_rows, const GemmRo
     for (int j = 0; j < T::kLoadsX; ++j) sox[j] = (uint32_t)j * x_rows.step;
     // (last: the load is of the last K step.)
     auto dma_w1 = [&](const i32x4& r, uint32_t stage, int j, bool last = false) __attribute__((always_inline)) {
-        dma1(r, kTailK && last ? w_rows.tail : dw, sow[j], lds_wave + stage, j);
+        gemm_dma(r, kTailK && last ? w_rows.tail : dw, sow[j], lds_wave + stage, j);
     };
     auto dma_x1 = [&](const i32x4& r, uint32_t stage, int j, bool last = false) __attribute__((always_inline)) {
-        dma1(r, kTailK && last ? x_rows.tail : dx, sox[j], lds_wave + T::kXBase + stage, j);
-    };
-    // The resource one K step further along its rows. The records stay: a
-    // lane's offset in its row is under 128 bytes and a row is at least the
-    // reduction long, so the row after the last one is out of range at every
-    // base.
-    auto advance = [](i32x4& r) __attribute__((always_inline)) {
-        const uint64_t base = ((uint64_t)(uint32_t)r.y << 32 | (uint32_t)r.x) + kPRow;
-        r.x = (int)(uint32_t)base;
-        r.y = (int)((uint32_t)(base >> 32) & 0xffffu);
+        gemm_dma(r, kTailK && last ? x_rows.tail : dx, sox[j], lds_wave + T::kXBase + stage, j);
     };
 
     // Fragment reads: lane l takes row (16*block + (l & 15)) of the wave's
@@ -223,11 +225,11 @@ __device__ __forceinline__ void gemm_k_loop(const GemmRows& w_rows, const GemmRo
         const int ix = i + 1 - SW + SX;
 #pragma unroll
         for (int j = 0; j < T::kLoadsW; ++j) dma_w1(i < nk ? rw : none, (uint32_t)(i * T::kWBytes), j, i == nk - 1);
-        advance(rw);
+        gemm_advance(rw);
         if (ix < 0) continue;
 #pragma unroll
         for (int j = 0; j < T::kLoadsX; ++j) dma_x1(ix < nk ? rx : none, (uint32_t)(ix * T::kXBytes), j, ix == nk - 1);
-        advance(rx);
+        gemm_advance(rx);
     }
 #pragma unroll
     for (int a = 0; a < T::NA; ++a)
@@ -275,8 +277,8 @@ __device__ __forceinline__ void gemm_k_loop(const GemmRows& w_rows, const GemmRo
             if constexpr (left >= SX)
                 spread(t, LoadsX{}, Most{}, [&](int i) __attribute__((always_inline)) { dma_x1(rx, cx, i, left == SX); });
         });
-        advance(rw);
-        advance(rx);
+        gemm_advance(rw);
+        gemm_advance(rx);
         pw = cw;
         cw = nw;
         cx = nx;

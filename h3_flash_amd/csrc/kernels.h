@@ -337,7 +337,10 @@ struct LinearFp8Params : LinearParams {
     int32_t w_blocks;        // ceil(n / 128)
     uint8_t* y_scale;        // e8m0 (m, ceil(n / 128)), NULL: y is bf16
     int64_t y_scale_rs;
-    float* y32;              // set by the launcher: the unrounded result, for its quantisation
+    // Set by the launcher: the unrounded result, for its rounding, and the sums of
+    // tiles in pieces.
+    float* y32;
+    void* sums;
 };
 // Chooses the form; *workspace: the bytes that it takes, *required: those that it
 // cannot do without (the others are the sums of tiles in pieces).
