@@ -22,7 +22,8 @@ LIB_PATH = LIB_DIR / "libh3attn.so"
 INCLUDE_DIR = REPO_DIR / "include"
 
 SOURCES = ("capi.hip", "attn_fwd.hip", "qknorm_rope.hip", "relayout.hip", "fusions.hip", "attn_merge.hip", "proj_gemm.hip", "clock.hip", "capi_block.hip", "linear.hip", "sandwich_norm.hip",
-           "block_select.hip", "attn_sparse.hip", "capi_fp8.hip", "quantize.hip", "modulate_fp8.hip", "linear_fp8.hip")
+           "block_select.hip", "attn_sparse.hip", "capi_fp8.hip", "quantize.hip", "modulate_fp8.hip", "linear_fp8.hip",
+           "linear_fp8_256x16.hip", "linear_fp8_256x12.hip", "linear_fp8_256x8.hip", "linear_fp8_128.hip")
 
 HIPCC_FLAGS = (
     "--offload-arch=gfx950",

@@ -59,8 +59,9 @@ int prepare_linear_fp8(const h3a_linear_fp8_args* a, h3a::LinearFp8Params& p, in
     if (a->weight_scale_stride >= kMaxSpan / (2 * groups_of(a->n)))
         return fail(H3A_EUNSUPPORTED, "%s: the scales of weight must span less than 2^31 bytes", fn);
     if (a->x_stride > (kMaxSpan - 1) / (x_size * rows) || a->weight_stride > (kMaxSpan - 1) / rows ||
-        (x8 && a->x_scale_stride > (kMaxSpan - 1) / rows))
-        return fail(H3A_EUNSUPPORTED, "%s: %lld rows of x and of weight must span less than 2^31 bytes", fn, (long long)rows);
+        a->y_stride > (kMaxSpan - 1) / ((y8 ? 1 : 2) * rows) || (a->residual != nullptr && a->residual_stride > (kMaxSpan - 1) / (2 * rows)) ||
+        (x8 && a->x_scale_stride > (kMaxSpan - 1) / rows) || (y8 && a->y_scale_stride > (kMaxSpan - 1) / rows))
+        return fail(H3A_EUNSUPPORTED, "%s: %lld rows of an operand must span less than 2^31 bytes", fn, (long long)rows);
     if ((rc = check_epilogue(fn, *a, p)) != H3A_OK) return rc;
     p.x = a->x; p.w = a->weight; p.y = a->y;
     p.x_rs = a->x_stride * x_size; p.w_rs = a->weight_stride; p.y_rs = a->y_stride * (y8 ? 1 : 2);

@@ -346,6 +346,11 @@ struct LinearFp8Params : LinearParams {
 // cannot do without (the others are the sums of tiles in pieces).
 void plan_linear_fp8(LinearFp8Params& p, int cus, int64_t* required, int64_t* workspace);
 hipError_t launch_linear_fp8(const LinearFp8Params& p, int cus, hipStream_t stream);
+// Of tiles of TF features (gated: value and gate rows) x 16 NT tokens, with SW and SX
+// stages of W and X; kLinearFp8MaxSplit: most pieces of a tile along k.
+template <int TF, int NT, int SW, int SX>
+hipError_t launch_linear_fp8_tile(const LinearFp8Params& p, hipStream_t stream);
+constexpr int kLinearFp8MaxSplit = 8;
 
 // Norm of a branch, gate, scaled residual, norm and modulation. Strides in elements.
 struct SandwichParams {

@@ -134,8 +134,8 @@ H3A_API int h3a_residual_gate_rmsnorm_modulate_fp8(const h3a_residual_gate_rmsno
  * sums over one instruction's 64 or 128 products are some 12 bits wide below the
  * largest product, and accumulated in fp32.
  * k is a positive multiple of 16, n of 8 (of 16 with y in 8 bits); rows are 16-byte
- * aligned; 256 rows of x and of weight, and all scales of weight, span less than 2^31
- * bytes. y may be the residual (bf16) and overlaps no other operand.
+ * aligned; 256 rows of an operand or result, and all scales of weight, span less than
+ * 2^31 bytes. y may be the residual (bf16) and overlaps no other operand.
  * Workspace: h3a_linear_fp8_workspace_size bytes, 256-byte aligned.
  * h3a_linear_fp8_required_workspace of them (x's or y's other form) it cannot do
  * without; with less than the whole, tiles are not cut along k. workspace NULL with
