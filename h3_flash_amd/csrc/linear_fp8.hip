@@ -29,12 +29,17 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 // bf16 rows of x are rounded to 8 bits as they come in: the four lanes of a row hold a
 // whole group.
 constexpr int kRowsMaxTokens = 32;
+// It serves small weights, where the call's latency counts. Larger ones come in faster
+// by the tiles' deep rings of loads, also for one block of 16 tokens and a launch more
+// that rounds bf16 rows (us, this form at its best / tiles: 16 x 5,376 x 5,376 12.4 /
+// 14.7; 16 x 14,336 x 5,376 26.2 / 20.4; 16 x 5,376 x 32,256 37.2 / 31.5; 32 x 1,024 x
+// 4,096 5.4 / 6.4; 32 x 5,376 x 5,376 16.8 / 15).
+constexpr int64_t kRowsMaxWeight[2] = {48 << 20, 16 << 20};  // bytes, up to 16 and 32 tokens
 constexpr int kRowsForm = -1, kNoForm = -2;  // in place of a tile shape
 
 template <int NA, int NB, bool kGated, bool kXBf16>
 __global__ __launch_bounds__(NA == 1 ? 1024 : 512) void linear_fp8_rows_kernel(LinearFp8Params p) {
     constexpr int kS = kGated ? 2 : 1, NF = NA / kS;  // blocks of output features
-    constexpr int kU = NA * NB >= 4 || kXBf16 ? 1 : 4;
     constexpr int kX = kXBf16 ? 4 : 2;  // 16-byte loads of a row's pieces
     extern __shared__ f32x4 part[];  // [wave][NA * NB][64]
     const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, l15 = lane & 15;
@@ -61,84 +66,76 @@ __global__ __launch_bounds__(NA == 1 ? 1024 : 512) void linear_fp8_rows_kernel(L
 #pragma unroll
         for (int b = 0; b < NB; ++b) acc[a][b] = f32x4{};
     const int chunks = (p.k + kFp8Group - 1) / kFp8Group;
-    for (int c0 = wave; c0 < chunks; c0 += waves * kU) {
-        i32x4 w[kU][2][NA], x[kU][kX][NB];
-        int sw[kU][kS], sx[kU][NB];
-        bool in[kU][2];
+    for (int c = wave; c < chunks; c += waves) {
+        i32x4 w[2][NA], x[kX][NB];
+        int sw[kS], sx[NB];
+        bool in[2];
 #pragma unroll
-        for (int u = 0; u < kU; ++u) {
-            const int c = c0 + u * waves;
+        for (int h = 0; h < 2; ++h) {
+            const int at = c * kFp8Group + h * 64 + q * 16;
+            in[h] = at < p.k;
+            const int o = in[h] ? at : p.k - 16;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int at = c * kFp8Group + h * 64 + q * 16;
-                in[u][h] = at < p.k;
-                const int o = in[u][h] ? at : p.k - 16;
-#pragma unroll
-                for (int a = 0; a < NA; ++a) w[u][h][a] = *(const i32x4*)(wr[a] + o);
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    if constexpr (kXBf16) {
-                        x[u][2 * h][b] = *(const i32x4*)(xr[b] + 2 * o);
-                        x[u][2 * h + 1][b] = *(const i32x4*)(xr[b] + 2 * o + 16);
-                    } else {
-                        x[u][h][b] = *(const i32x4*)(xr[b] + o);
-                    }
-                }
-            }
-            const int cs = min(c, chunks - 1);
-#pragma unroll
-            for (int s = 0; s < kS; ++s) sw[u][s] = ws[s][cs];
-            if constexpr (!kXBf16) {
-#pragma unroll
-                for (int b = 0; b < NB; ++b) sx[u][b] = xs[b][cs];
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < kU; ++u) {
-            i32x8 xv[NB];
+            for (int a = 0; a < NA; ++a) w[h][a] = *(const i32x4*)(wr[a] + o);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 if constexpr (kXBf16) {
-                    float v[4][8];
-                    uint32_t top = 0;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const i32x4 raw = in[u][i / 2] ? x[u][i][b] : i32x4{};
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            v[i][2 * e] = __uint_as_float((uint32_t)raw[e] << 16);
-                            v[i][2 * e + 1] = __uint_as_float((uint32_t)raw[e] & 0xffff0000u);
-                        }
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[i][e]) & 0x7fffffffu);
-                    }
-                    top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
-                    top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
-                    sx[u][b] = fp8_exponent(top);
-                    const float inv = fp8_inverse(sx[u][b]);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        xv[b][2 * i] = fp8x4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
-                        xv[b][2 * i + 1] = fp8x4(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv);
-                    }
+                    x[2 * h][b] = *(const i32x4*)(xr[b] + 2 * o);
+                    x[2 * h + 1][b] = *(const i32x4*)(xr[b] + 2 * o + 16);
                 } else {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) xv[b][4 * h + e] = in[u][h] ? x[u][h][b][e] : 0;
+                    x[h][b] = *(const i32x4*)(xr[b] + o);
                 }
             }
+        }
 #pragma unroll
-            for (int a = 0; a < NA; ++a) {
-                i32x8 wv;
+        for (int s = 0; s < kS; ++s) sw[s] = ws[s][c];
+        if constexpr (!kXBf16) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b) sx[b] = xs[b][c];
+        }
+        i32x8 xv[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            if constexpr (kXBf16) {
+                float v[4][8];
+                uint32_t top = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const i32x4 raw = in[i / 2] ? x[i][b] : i32x4{};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        v[i][2 * e] = __uint_as_float((uint32_t)raw[e] << 16);
+                        v[i][2 * e + 1] = __uint_as_float((uint32_t)raw[e] & 0xffff0000u);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[i][e]) & 0x7fffffffu);
+                }
+                top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+                top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+                sx[b] = fp8_exponent(top);
+                const float inv = fp8_inverse(sx[b]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    xv[b][2 * i] = fp8x4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
+                    xv[b][2 * i + 1] = fp8x4(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv);
+                }
+            } else {
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) wv[4 * h + e] = in[u][h] ? w[u][h][a][e] : 0;
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-                    acc[a][b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, xv[b], acc[a][b], 0, 0, 0, sw[u][a % kS], 0, sx[u][b]);
+                    for (int e = 0; e < 4; ++e) xv[b][4 * h + e] = in[h] ? x[h][b][e] : 0;
             }
+        }
+#pragma unroll
+        for (int a = 0; a < NA; ++a) {
+            i32x8 wv;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) wv[4 * h + e] = in[h] ? w[h][a][e] : 0;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+                acc[a][b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, xv[b], acc[a][b], 0, 0, 0, sw[a % kS], 0, sx[b]);
         }
     }
 #pragma unroll
@@ -182,7 +179,7 @@ struct RowsForm {
 RowsForm rows_form(const LinearFp8Params& p, int cus) {
     const int64_t blocks = (int64_t)((p.n + 15) / 16) * (p.gated ? 2 : 1);
     RowsForm f;
-    f.na = blocks >= 4ll * cus ? 4 : blocks >= cus || p.gated ? 2 : 1;
+    f.na = blocks >= 4ll * cus ? 4 : blocks > cus || p.gated ? 2 : 1;
     f.groups = (blocks + f.na - 1) / f.na;
     f.waves = 4;
     while (f.waves < (f.na == 1 ? 16 : 8) && f.groups * f.waves < 16ll * cus && f.waves * kFp8Group < p.k) f.waves *= 2;
@@ -201,20 +198,26 @@ hipError_t launch_rows(const LinearFp8Params& p, int cus, hipStream_t stream) {
 // ---------------------------------------------------------------- tiles
 
 // The tile shapes, with the time of a K step of 128 with all CUs busy and a tile's
-// fixed part (launch, first loads, epilogue).
+// fixed part (launch, first loads, epilogue). Fitted to graph replays of 26 sizes (16
+// to 12,480 tokens, 2,048 to 32,256 features, k 1,552 to 14,336) in every shape and
+// split; the choice by them takes 0.5% longer than the best of all, in the mean.
 struct Shape {
     int tf, nt;
     float step_us, fixed_us;
     hipError_t (*launch)(const LinearFp8Params&, hipStream_t);
 };
 constexpr Shape kShapes[] = {
-    {256, 16, 1.36f, 13.3f, launch_linear_fp8_tile<256, 16, 3, 2>}, {256, 12, 1.05f, 11.8f, launch_linear_fp8_tile<256, 12, 3, 2>}, {256, 8, 0.80f, 9.3f, launch_linear_fp8_tile<256, 8, 3, 3>},
-    {128, 8, 0.50f, 5.9f, launch_linear_fp8_tile<128, 8, 5, 4>},    {128, 6, 0.40f, 5.9f, launch_linear_fp8_tile<128, 6, 6, 4>},
-    {128, 4, 0.34f, 5.3f, launch_linear_fp8_tile<128, 4, 6, 5>},    {128, 2, 0.27f, 3.6f, launch_linear_fp8_tile<128, 2, 8, 6>},
+    {256, 16, 1.352f, 6.57f, launch_linear_fp8_tile<256, 16, 3, 2>}, {256, 12, 1.034f, 6.07f, launch_linear_fp8_tile<256, 12, 3, 2>},
+    {256, 8, 0.795f, 5.18f, launch_linear_fp8_tile<256, 8, 3, 3>},   {128, 8, 0.485f, 4.84f, launch_linear_fp8_tile<128, 8, 5, 4>},
+    {128, 6, 0.375f, 4.98f, launch_linear_fp8_tile<128, 6, 6, 4>},   {128, 4, 0.317f, 5.74f, launch_linear_fp8_tile<128, 4, 6, 5>},
+    {128, 2, 0.295f, 2.95f, launch_linear_fp8_tile<128, 2, 8, 6>},
 };
-constexpr float kIdleGain = 0.36f;  // of a K step's time, saved as the CUs of a round go idle
-// A second launch joins the pieces, over their sums at 0.32 us a MB.
-constexpr float kJoinUs = 1.9f, kJoinUsPerByte = 0.32e-6f;
+constexpr float kIdleGain = 0.29f;  // of a K step's time, saved as the CUs of a round go idle
+// A second launch joins the pieces, over their sums at 0.24 us a MB.
+constexpr float kJoinUs = 2.13f, kJoinUsPerByte = 0.24e-6f;
+// The operands from memory; of this and the tiles' time the larger counts, and a tenth
+// of the smaller.
+constexpr float kMemoryUs = 7.2f, kMemoryUsPerByte = 1.0f / 7.52e6f;
 constexpr int kSplits[] = {2, 3, 4, 6, kLinearFp8MaxSplit};
 constexpr int kMinPieceSteps = 8;
 
@@ -254,7 +257,8 @@ void plan_linear_fp8(LinearFp8Params& p, int cus, int64_t* required, int64_t* wo
     if (cus <= 0) cus = 256;
     *required = *workspace = 0;
     p.shape = kNoForm;
-    if (p.m <= kRowsMaxTokens) {
+    const int64_t w_bytes = (p.gated ? 2 : 1) * (int64_t)p.n * p.k;
+    if (p.m <= kRowsMaxTokens && w_bytes <= kRowsMaxWeight[p.m > 16]) {
         const RowsForm f = rows_form(p, cus);
         if (f.groups * 64 * f.waves <= UINT32_MAX) p.shape = kRowsForm;  // work items of a launch
         if (p.y_scale != nullptr) *required = *workspace = 4 * (int64_t)p.m * p.n;
@@ -265,6 +269,7 @@ void plan_linear_fp8(LinearFp8Params& p, int cus, int64_t* required, int64_t* wo
         if ((int64_t)p.m * ((p.k + kFp8Group - 1) / kFp8Group) >= (int64_t)1 << 30) return;  // as h3a_quantize_fp8
     }
     const int steps = (p.k + kFp8Group - 1) / kFp8Group;
+    const float memory_us = kMemoryUs + kMemoryUsPerByte * ((float)w_bytes + (float)p.m * (float)p.k + 2.f * (float)p.m * (float)p.n);
     float best_us = 0.f;
     for (int i = 0; i < (int)(sizeof(kShapes) / sizeof(kShapes[0])); ++i) {
         const Shape& s = kShapes[i];
@@ -293,6 +298,7 @@ void plan_linear_fp8(LinearFp8Params& p, int cus, int64_t* required, int64_t* wo
                 split = n;
             }
         }
+        us = us > memory_us ? us + 0.1f * memory_us : memory_us + 0.1f * us;
         if (p.shape >= 0 && us >= best_us) continue;
         best_us = us;
         p.shape = i;

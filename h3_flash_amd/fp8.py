@@ -23,7 +23,7 @@ from __future__ import annotations
 import torch
 
 from . import _ext
-from .fusions import _aligned_rows, _dtype, _fp8_scales, _index, _index_args, _tables, _vector
+from .fusions import _aligned_rows, _dtype, _empty, _fp8_scales, _index, _index_args, _tables, _vector
 from .linear import _operand
 
 __all__ = ["fused_linear_fp8", "quantize_fp8", "quantize_fp8_weight"]
@@ -79,7 +79,7 @@ def _quantize(x: torch.Tensor, name: str, scale_rows: tuple[int, ...], block_row
     if columns == 0 or columns % 16:
         raise ValueError(f"{name}'s last dimension must be a positive multiple of 16, got {columns}")
     held, rows, stride = _held_rows(x, columns)
-    q = torch.empty(x.shape, dtype=E4M3, device=x.device)
+    q = _empty(x.shape, E4M3, x.device)
     scale, pitch = _fp8_scales(scale_rows, columns, x.device)
     if rows:
         _ext.quantize_fp8.run(
@@ -211,10 +211,10 @@ def fused_linear_fp8(
     if quantize:
         if out is not None:
             raise ValueError("quantize and out exclude each other")
-        y = out = torch.empty(shape, dtype=E4M3, device=device)
+        y = out = _empty(shape, E4M3, device)
         y_scale, ys_stride = _fp8_scales(shape[:-1], n, device)
     elif out is None:
-        y = out = torch.empty(shape, dtype=torch.bfloat16, device=device)
+        y = out = _empty(shape, torch.bfloat16, device)
     else:
         if out.shape != shape or out.dtype != torch.bfloat16 or out.device != device:
             raise ValueError(f"out must be a bf16 {shape} tensor on {device}")

@@ -99,14 +99,24 @@ def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
+def _empty(shape: tuple[int, ...], dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    """A contiguous empty tensor (of a matrix by its strides: half the call's time)."""
+
+    if len(shape) == 2:
+        return torch.empty_strided(shape, (max(shape[1], 1), 1), dtype=dtype, device=device)
+    return torch.empty(shape, dtype=dtype, device=device)
+
+
 def _fp8_scales(lead: tuple[int, ...], columns: int, device: torch.device) -> tuple[torch.Tensor, int]:
     """An empty (*lead, ceil(columns / 128)) tensor of e8m0 scales whose rows start at
     multiples of 16 bytes, and their stride."""
 
     groups = (columns + 127) // 128
     pitch = (groups + 15) // 16 * 16
-    scale = torch.empty((*lead, pitch), dtype=torch.float8_e8m0fnu, device=device)
-    return (scale if pitch == groups else scale[..., :groups]), pitch
+    scale = _empty((*lead, pitch), torch.float8_e8m0fnu, device)
+    if pitch == groups:
+        return scale, pitch
+    return (scale.as_strided((lead[0], groups), (pitch, 1)) if len(lead) == 1 else scale[..., :groups]), pitch
 
 
 def _norm_operand(x: torch.Tensor, name: str, columns: int) -> tuple[torch.Tensor, int, int]:
@@ -262,7 +272,7 @@ def fused_rmsnorm_modulate_fp8(x, weight, scale, shift, index, eps):
     held, rows, stride = _norm_operand(x, "x", columns)
     weight, tables, index = _norm_fp8_args(weight, [scale, shift], index, columns, device)
     scale, shift = tables
-    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=device)
+    q = _empty(x.shape, torch.float8_e4m3fn, device)
     q_scale, pitch = _fp8_scales(x.shape[:-1], columns, device)
     _ext.rmsnorm_modulate_fp8.run(
         device, _ext.ABI_VERSION, held.data_ptr(), q.data_ptr(), q_scale.data_ptr(), weight.data_ptr(), _dtype(weight),
@@ -287,8 +297,7 @@ def fused_residual_gate_rmsnorm_modulate_fp8(residual, branch, gate, weight, sca
         raise ValueError(f"residual and branch must be on one device, got {device} and {branch.device}")
     weight, tables, index = _norm_fp8_args(weight, [gate, scale, shift], index, columns, device)
     gate, scale, shift = tables
-    hidden = torch.empty(residual.shape, dtype=torch.bfloat16, device=device)
-    q = torch.empty(residual.shape, dtype=torch.float8_e4m3fn, device=device)
+    hidden, q = _empty(residual.shape, torch.bfloat16, device), _empty(residual.shape, torch.float8_e4m3fn, device)
     q_scale, pitch = _fp8_scales(residual.shape[:-1], columns, device)
     _ext.residual_gate_rmsnorm_modulate_fp8.run(
         device, _ext.ABI_VERSION, rows_r.data_ptr(), rows_b.data_ptr(), hidden.data_ptr(), q.data_ptr(), q_scale.data_ptr(),
