@@ -63,6 +63,7 @@ int prepare_linear_fp8(const h3a_linear_fp8_args* a, h3a::LinearFp8Params& p, in
         (x8 && a->x_scale_stride > (kMaxSpan - 1) / rows) || (y8 && a->y_scale_stride > (kMaxSpan - 1) / rows))
         return fail(H3A_EUNSUPPORTED, "%s: %lld rows of an operand must span less than 2^31 bytes", fn, (long long)rows);
     if ((rc = check_epilogue(fn, *a, p)) != H3A_OK) return rc;
+    if (p.table_rows >= (int64_t)1 << 31) return fail(H3A_EUNSUPPORTED, "%s: the gate's table must have fewer than 2^31 rows", fn);
     p.x = a->x; p.w = a->weight; p.y = a->y;
     p.x_rs = a->x_stride * x_size; p.w_rs = a->weight_stride; p.y_rs = a->y_stride * (y8 ? 1 : 2);
     p.x_scale = x8 ? (const uint8_t*)a->x_scale : nullptr;

@@ -61,8 +61,8 @@ struct Fp8Tile {
     static constexpr bool kEarlyX = TF == 256;
     static constexpr int kLds = kStages + kSegs * kSegBytes;
     // Blocks of tokens of a wave that the epilogue takes at a time: all, or what fits.
-    static constexpr int kPass = kTokens * TF * 4 <= 160 * 1024 ? NB : NB % 2 == 0 ? NB / 2 : 1;
-    static constexpr int kEpiBytes = 32 * kPass * WM * TF * 4;
+    static constexpr int kPass = kTokens * (TF + 1) * 4 <= 160 * 1024 ? NB : NB % 2 == 0 ? NB / 2 : 1;
+    static constexpr int kEpiRows = 32 * kPass * WM * TF * 4, kEpiBytes = kEpiRows + kTokens * 4;
     static constexpr int kSmem = kLds > kEpiBytes ? kLds : kEpiBytes;
     static_assert(NT % 2 == 0 && TF % 128 == 0, "DMA map: whole loads per wave");
     static_assert(NA * WN * 32 == TF && 2 * NB * WM == NT && NB % kPass == 0, "wave map");

@@ -12,6 +12,7 @@ namespace h3a {
 namespace {
 
 typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
+typedef __attribute__((address_space(3))) int lds_i32;
 
 // Maximum over aligned groups of 32 lanes; all lanes must be active.
 __device__ __forceinline__ uint32_t group32_max(uint32_t v) {
@@ -28,11 +29,17 @@ __device__ __forceinline__ int64_t gate_row32(const LinearFp8Params& p, int m) {
     return t >= p.table_rows ? p.table_rows - 1 : t;
 }
 
-// SiLU where nothing else is asked for: activate()'s with the bound that keeps -inf
-// at its limit (NaN stays).
+// SiLU where nothing else is asked for. (-inf comes to its limit -0; NaN stays in s.)
 __device__ __forceinline__ float silu(float z) {
     const float s = __builtin_amdgcn_rcpf(1.0f + fast_exp2(z * -1.44269504088896f));
-    return (z < -1e12f ? -1e12f : z) * s;
+    return fmaxf(z, -1e30f) * s;
+}
+
+// Bits of the largest magnitude of four values.
+__device__ __forceinline__ uint32_t top4(const f32x4& y) {
+    // (maximum keeps NaN, and takes magnitudes at no cost)
+    const float a = __builtin_elementwise_maximum(__builtin_elementwise_maximum(fabsf(y[0]), fabsf(y[1])), fabsf(y[2]));
+    return __float_as_uint(__builtin_elementwise_maximum(a, fabsf(y[3]))) & 0x7fffffffu;
 }
 
 // Epilogue of a tile: lane l holds, for token block b (token 32 (NB wm + b) + (l & 31)),
@@ -42,10 +49,11 @@ __device__ __forceinline__ float silu(float z) {
 // c ^ (r & 7), and a thread then takes four features of a token at a time, kBatch
 // tokens in flight. In 8 bits, 32 neighbouring threads hold a group of 128 features.
 // Rows past m and features past n are outside the records of the result's (and the
-// residual's) buffer, so that no branch breaks up a batch, and one without gate and
-// residual has a loop of its own. (With a branch per token for each of them, as
-// linear.hip has it, the epilogue took 25,400 of the 129,500 cycles of a 256 x 256
-// tile of k = 5,120, and 32,800 of 140,700 gated, in 8 bits, at k = 5,376.)
+// residual's) buffer, so that no branch breaks up a batch; without a bias, gate or
+// residual, and with a bias alone, the loop has a form of its own. (With a branch per
+// token for each of them, as linear.hip has it, the epilogue took 25,400 of the 129,500
+// cycles of a 256 x 256 tile of k = 5,120, and 32,800 of 140,700 gated, in 8 bits, at
+// k = 5,376.) The tokens' gate rows are looked up once, into LDS behind the rows.
 template <typename T, bool kGated, bool kQuant>
 __device__ __forceinline__ void linear_fp8_epilogue(const LinearFp8Params& p, int f0, int m0, const f32x16 (&acc)[T::NA][T::NB],
                                                     int wn, int wm, int tid, char* smem) {
@@ -72,6 +80,8 @@ __device__ __forceinline__ void linear_fp8_epilogue(const LinearFp8Params& p, in
                                   p.residual != nullptr ? (uint32_t)((rows - 1) * p.res_rs + 2 * (int64_t)p.n) : 0u);
     const uint32_t r_off = in ? (uint32_t)(r0 * p.res_rs + 2 * f) : kOut;
     lds_char* const buf = (lds_char*)smem;
+    lds_i32* const gate_rows = (lds_i32*)(buf + T::kEpiRows);
+    if (p.gate != nullptr && tid < T::kTokens) gate_rows[tid] = (int)gate_row32(p, min(m0 + tid, p.m - 1));  // (read after the pass's barrier)
     lds_char* const wr = buf + (wm * kRowsPass + (lane & 31)) * kRowBytes;
     const int sw = lane & 7;
     auto pass = [&](auto h_c) __attribute__((always_inline)) {
@@ -94,27 +104,30 @@ __device__ __forceinline__ void linear_fp8_epilogue(const LinearFp8Params& p, in
         auto first_token = [&](int j) __attribute__((always_inline)) {
             return (T::WM == 2 ? j / kPerWave : 0) * (32 * T::NB) + 32 * b0 + (T::WM == 2 ? j % kPerWave : j) * (kBatch * kRows);
         };
-        auto loop = [&](auto act, auto plain_c) __attribute__((always_inline)) {
-            constexpr bool kPlain = decltype(plain_c)::value;
+        // kMode 0: nothing but the activation; 1: a bias; 2: any of bias, gate, residual.
+        auto loop = [&](auto act, auto mode_c) __attribute__((always_inline)) {
+            constexpr int kMode = decltype(mode_c)::value;
             struct Batch {
                 i32x2 res[kBatch];
                 f32x4 gate[kBatch];
             };
             auto load_batch = [&](Batch& q, int j) __attribute__((always_inline)) {
                 const int t0 = first_token(j);
+                if (p.residual != nullptr) {
 #pragma unroll
-                for (int i = 0; i < kBatch; ++i)
-                    q.res[i] = __builtin_amdgcn_raw_buffer_load_b64(r_rsrc, (int)r_off, (int)((t0 + kRows * i) * p.res_rs), 0);
+                    for (int i = 0; i < kBatch; ++i)
+                        q.res[i] = __builtin_amdgcn_raw_buffer_load_b64(r_rsrc, (int)r_off, (int)((t0 + kRows * i) * p.res_rs), 0);
+                }
                 if (p.gate != nullptr) {
-                    int64_t at[kBatch];
+                    const char* at[kBatch];
 #pragma unroll
-                    for (int i = 0; i < kBatch; ++i) at[i] = gate_row32(p, min(m0 + t0 + r0 + kRows * i, p.m - 1)) * p.gate_rs;
+                    for (int i = 0; i < kBatch; ++i) at[i] = (const char*)p.gate + gate_rows[t0 + r0 + kRows * i] * p.gate_rs;
                     if (p.gate_f32) {
 #pragma unroll
-                        for (int i = 0; i < kBatch; ++i) q.gate[i] = *(const f32x4*)((const char*)p.gate + at[i] + 4 * fc);
+                        for (int i = 0; i < kBatch; ++i) q.gate[i] = *(const f32x4*)(at[i] + 4 * fc);
                     } else {
 #pragma unroll
-                        for (int i = 0; i < kBatch; ++i) q.gate[i] = unpack4(*(const i32x2*)((const char*)p.gate + at[i] + 2 * fc));
+                        for (int i = 0; i < kBatch; ++i) q.gate[i] = unpack4(*(const i32x2*)(at[i] + 2 * fc));
                     }
                 } else {
 #pragma unroll
@@ -122,11 +135,11 @@ __device__ __forceinline__ void linear_fp8_epilogue(const LinearFp8Params& p, in
                 }
             };
             Batch cur;
-            if constexpr (!kPlain) load_batch(cur, 0);
+            if constexpr (kMode == 2) load_batch(cur, 0);
 #pragma unroll 1
             for (int j = 0; j < T::WM * kPerWave; ++j) {
                 Batch next;
-                if constexpr (!kPlain)
+                if constexpr (kMode == 2)
                     if (j + 1 < T::WM * kPerWave) load_batch(next, j + 1);
                 const int t0 = first_token(j), l0 = j * (kBatch * kRows) + r0;
                 f32x4 z[kBatch][kS];
@@ -136,54 +149,63 @@ __device__ __forceinline__ void linear_fp8_epilogue(const LinearFp8Params& p, in
                     for (int s = 0; s < kS; ++s) {
                         const int r = l0 + kRows * i;
                         z[i][s] = *(const lds_f32x4*)(buf + r * kRowBytes + (((s * kCols + c) ^ (r & 7)) << 4));
+                        if constexpr (kMode > 0) z[i][s] += bias[s];
                     }
+                f32x4 y[kBatch];
 #pragma unroll
                 for (int i = 0; i < kBatch; ++i) {
-                    f32x4 y;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        y[e] = act(z[i][kS - 1][e] + bias[kS - 1][e]);
-                        if constexpr (kGated) y[e] *= z[i][0][e] + bias[0][e];
+                        y[i][e] = act(z[i][kS - 1][e]);
+                        if constexpr (kGated) y[i][e] *= z[i][0][e];
                     }
-                    if constexpr (!kPlain) {
-                        y *= cur.gate[i];
-                        if (p.residual != nullptr) y += unpack4(cur.res[i]);
-                    }
-                    const int row = t0 + kRows * i;
-                    if constexpr (kQuant) {
-                        uint32_t top = 0;
+                    if constexpr (kMode == 2) y[i] *= cur.gate[i];
+                }
+                if constexpr (kMode == 2) {
+                    if (p.residual != nullptr) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(y[e]) & 0x7fffffffu);
-                        const int s = fp8_exponent(group32_max(in ? top : 0));
-                        const float inv = fp8_inverse(s);
-                        __builtin_amdgcn_raw_buffer_store_b32(fp8x4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv), y_rsrc, (int)y_off,
-                                                              (int)(row * p.y_rs), 0);
-                        __builtin_amdgcn_raw_buffer_store_b8((uint8_t)s, s_rsrc, (int)s_off, (int)(row * p.y_scale_rs), 0);
-                    } else {
-                        __builtin_amdgcn_raw_buffer_store_b64(i32x2{(int)pack_bf16x2(y[0], y[1]), (int)pack_bf16x2(y[2], y[3])}, y_rsrc, (int)y_off,
-                                                              (int)(row * p.y_rs), 0);
+                        for (int i = 0; i < kBatch; ++i) y[i] += unpack4(cur.res[i]);
                     }
                 }
-                if constexpr (!kPlain) cur = next;
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) {
+                    const int row = t0 + kRows * i;
+                    if constexpr (kQuant) {
+                        const int s = fp8_exponent(group32_max(in ? top4(y[i]) : 0));
+                        const float inv = fp8_inverse(s);
+                        __builtin_amdgcn_raw_buffer_store_b32(fp8x4(y[i][0] * inv, y[i][1] * inv, y[i][2] * inv, y[i][3] * inv), y_rsrc,
+                                                              (int)y_off, (int)(row * p.y_rs), 0);
+                        __builtin_amdgcn_raw_buffer_store_b8((uint8_t)s, s_rsrc, (int)s_off, (int)(row * p.y_scale_rs), 0);
+                    } else {
+                        __builtin_amdgcn_raw_buffer_store_b64(i32x2{(int)pack_bf16x2(y[i][0], y[i][1]), (int)pack_bf16x2(y[i][2], y[i][3])}, y_rsrc,
+                                                              (int)y_off, (int)(row * p.y_rs), 0);
+                    }
+                }
+                if constexpr (kMode == 2) cur = next;
             }
         };
-        // One copy of the loop per activation: its code is what runs.
-        auto either = [&](auto act) __attribute__((always_inline)) {
-            if (p.gate == nullptr && p.residual == nullptr)
-                loop(act, std::true_type{});
+        // One copy of the loop per activation (with gate or residual, two activations
+        // share one): its code is what runs.
+        auto with = [&](auto mode) __attribute__((always_inline)) {
+            if (p.act == H3A_ACT_NONE)
+                loop([](float z) { return z; }, mode);
+            else if (p.act == H3A_ACT_RELU)
+                loop([](float z) { return activate(z, H3A_ACT_RELU); }, mode);
+            else if (p.act == H3A_ACT_GELU)
+                loop([](float z) { return activate(z, H3A_ACT_GELU); }, mode);
+            else if constexpr (decltype(mode)::value == 2)
+                loop([&](float z) { return activate(z, p.act == H3A_ACT_SILU ? H3A_ACT_SILU : H3A_ACT_GELU_TANH); }, mode);
+            else if (p.act == H3A_ACT_SILU)
+                loop([](float z) { return silu(z); }, mode);
             else
-                loop(act, std::false_type{});
+                loop([](float z) { return activate(z, H3A_ACT_GELU_TANH); }, mode);
         };
-        if (p.act == H3A_ACT_NONE)
-            either([](float z) { return z; });
-        else if (p.act == H3A_ACT_RELU)
-            either([](float z) { return activate(z, H3A_ACT_RELU); });
-        else if (p.act == H3A_ACT_GELU)
-            either([](float z) { return activate(z, H3A_ACT_GELU); });
-        else if (p.act == H3A_ACT_SILU)
-            either([](float z) { return silu(z); });
+        if (p.gate != nullptr || p.residual != nullptr)
+            with(std::integral_constant<int, 2>{});
+        else if (p.bias != nullptr)
+            with(std::integral_constant<int, 1>{});
         else
-            either([](float z) { return activate(z, H3A_ACT_GELU_TANH); });
+            with(std::integral_constant<int, 0>{});
     };
     static_for<T::NB / T::kPass>(pass);
 }
