@@ -310,6 +310,7 @@ __device__ __forceinline__ void gemm_fp8_k_loop(const GemmRows& w_rows, const Ge
     // use the one before it, but for the last block, which comes first here; after a
     // barrier the step's X stage is loaded again in the first half, its W stage in the
     // second.
+    // (The last reads of a half go out a few MFMAs before its end, which waits for them.)
     // `left` K steps follow; the last steps run out of loads, the last one reads nothing.
     uint32_t cw = 0, pw = (SW - 1) * T::kWBytes, cx = 0;
     int kt = 0;
@@ -350,7 +351,7 @@ __device__ __forceinline__ void gemm_fp8_k_loop(const GemmRows& w_rows, const Ge
                     asm volatile("" : "+v"(fx[1][T::NB - 1]));  // (read)
                     barrier();
                 }
-                spread(t, H3A_C(2 * T::NA), H3A_C(kXAt), H3A_C(kMfmas), [&](int i) __attribute__((always_inline)) { read_w(cw, 1, i >> 1, i & 1); });
+                spread(t, H3A_C(2 * T::NA), H3A_C(kXAt), H3A_C(kMfmas - 3), [&](int i) __attribute__((always_inline)) { read_w(cw, 1, i >> 1, i & 1); });
                 if constexpr (left >= SX)
                     spread(t, H3A_C(T::kLoadsX), H3A_C(kXAt), H3A_C(kMfmas), [&](int i) __attribute__((always_inline)) { dma_x1(cx, i, left == SX); });
             } else {
@@ -371,7 +372,7 @@ __device__ __forceinline__ void gemm_fp8_k_loop(const GemmRows& w_rows, const Ge
             // (The scales first: the next step's first MFMA needs them all.)
             constexpr int kFirst = kScales;
             if constexpr (left > 0) {
-                spread(t, H3A_C(kReads + kFirst), H3A_C(0), H3A_C(kMfmas), [&](int i) __attribute__((always_inline)) {
+                spread(t, H3A_C(kReads + kFirst), H3A_C(0), H3A_C(kEarlyX ? kMfmas - 2 : kMfmas), [&](int i) __attribute__((always_inline)) {
                     if (i >= kFirst)
                         read1(nw, nx, 0, i - kFirst);
                     else
