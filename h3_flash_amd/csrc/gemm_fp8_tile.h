@@ -43,7 +43,9 @@ template <int TF, int NT, int SW, int SX>
 struct Fp8Tile {
     static constexpr int kSW = SW, kSX = SX, kTF = TF;
     static constexpr int kTokens = 16 * NT;
-    static constexpr int WN = TF == 256 && NT >= 10 ? 2 : 4, WM = kPWaves / WN;
+    // Waves over features and tokens: the smaller side of what they read of LDS per MFMA.
+    // (128 x 128: 2 x 2, 22.2 us at 390 x 5,376 x 5,376, 22.8 by 4 x 1.)
+    static constexpr int WN = (TF == 256 && NT >= 10) || (TF == 128 && NT == 8) ? 2 : 4, WM = kPWaves / WN;
     static constexpr int NA = TF / 32 / WN, NB = NT / 2 / WM;  // 32 x 32 MFMA blocks of a wave
     static constexpr int kWBytes = TF * kPRow, kXBytes = kTokens * kPRow;
     static constexpr int kXBase = SW * kWBytes, kStages = kXBase + SX * kXBytes;

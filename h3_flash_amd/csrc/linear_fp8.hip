@@ -208,7 +208,7 @@ struct Shape {
 };
 constexpr Shape kShapes[] = {
     {256, 16, 1.352f, 6.57f, launch_linear_fp8_tile<256, 16, 3, 2>}, {256, 12, 1.034f, 6.07f, launch_linear_fp8_tile<256, 12, 3, 2>},
-    {256, 8, 0.795f, 5.18f, launch_linear_fp8_tile<256, 8, 3, 3>},   {128, 8, 0.485f, 4.84f, launch_linear_fp8_tile<128, 8, 5, 4>},
+    {256, 8, 0.795f, 5.18f, launch_linear_fp8_tile<256, 8, 3, 3>},   {128, 8, 0.472f, 4.78f, launch_linear_fp8_tile<128, 8, 5, 4>},
     {128, 6, 0.375f, 4.98f, launch_linear_fp8_tile<128, 6, 6, 4>},   {128, 4, 0.317f, 5.74f, launch_linear_fp8_tile<128, 4, 6, 5>},
     {128, 2, 0.295f, 2.95f, launch_linear_fp8_tile<128, 2, 8, 6>},
 };
