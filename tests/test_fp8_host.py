@@ -190,6 +190,14 @@ INVALID, UNSUPPORTED = _ext.H3A_EINVAL, _ext.H3A_EUNSUPPORTED
         ("h3a_linear_fp8", _linear(weight_stride=1 << 23), UNSUPPORTED, "2^31"),
         ("h3a_linear_fp8", _linear(x_dtype=0, x_stride=1 << 22), UNSUPPORTED, "2^31"),
         ("h3a_linear_fp8", _linear(x_scale_stride=1 << 23), UNSUPPORTED, "2^31"),
+        ("h3a_linear_fp8", _linear(n=1 << 20, y_stride=1 << 20, weight_scale_stride=1 << 17), UNSUPPORTED, "scales of weight"),
+        ("h3a_linear_fp8", _linear(y_stride=1 << 22), UNSUPPORTED, "2^31"),
+        ("h3a_linear_fp8", _linear8(y_stride=1 << 23), UNSUPPORTED, "2^31"),
+        ("h3a_linear_fp8", _linear8(y_scale_stride=1 << 23), UNSUPPORTED, "2^31"),
+        ("h3a_linear_fp8", _linear(residual=P, residual_stride=1 << 22), UNSUPPORTED, "2^31"),
+        ("h3a_linear_fp8", _linear(gate=P, gate_stride=32, table_rows=1 << 31, index=P, index_dtype=3, n_index=1), UNSUPPORTED, "2^31 rows"),
+        ("h3a_linear_fp8", _linear(n=1 << 30), UNSUPPORTED, "too large"),
+        ("h3a_linear_fp8", _linear(k=1 << 30), UNSUPPORTED, "too large"),
         ("h3a_linear_fp8", _linear(m=1 << 30, n=1 << 14, y_stride=1 << 14), UNSUPPORTED, "grid too large"),
         ("h3a_linear_fp8", _linear(bias=P, bias_dtype=2), INVALID, "bias dtype"),
         ("h3a_linear_fp8", _linear(bias=P + 8), INVALID, "bias"),

@@ -4,10 +4,12 @@ and over more than 2^31 values."""
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
-from h3_flash_amd import fused_linear, fused_linear_fp8, quantize_fp8, quantize_fp8_weight
+from h3_flash_amd import _ext, fused_linear, fused_linear_fp8, quantize_fp8, quantize_fp8_weight
 from h3_flash_amd.fusions import fused_residual_gate_rmsnorm_modulate, fused_residual_gate_rmsnorm_modulate_fp8, fused_rmsnorm_modulate_fp8
 from oracle.fp8 import dequantized
 from test_gpu_fp8 import BF16, DEV, _activations, _check, _randn, _same
@@ -131,6 +133,30 @@ def test_two_graphs_of_one_pool_and_two_streams():
                 outs[i].append(fused_linear_fp8(xs[i], *w))
     torch.cuda.synchronize()
     assert all(torch.equal(y, want[i]) for i in (0, 1) for y in outs[i])
+
+
+@pytest.mark.parametrize("x8", [False, True])
+def test_the_c_call_with_less_than_the_whole_workspace(x8):
+    # pieces along k where it fits, whole tiles where it does not, nothing behind it written
+    m, k, n = 200, 8208, 1032
+    x, (w, ws) = _activations(m, k, 1), quantize_fp8_weight(_randn(n, k, seed=2, scale=0.01))
+    q, s = quantize_fp8(x)
+    lib = _ext.load_library()
+    for short in (False, True):
+        y = torch.full((m + 3, n), 7.0, dtype=BF16, device=DEV)
+        of_x = dict(x=q.data_ptr(), x_dtype=4, x_scale=s.data_ptr(), x_scale_stride=s.stride(0)) if x8 else dict(x=x.data_ptr(), x_dtype=0)
+        args = _ext.LinearFp8Args(abi_version=_ext.ABI_VERSION, weight=w.data_ptr(), weight_scale=ws.data_ptr(), y=y.data_ptr(), y_dtype=0, m=m,
+                                  k=k, n=n, x_stride=k, weight_stride=k, weight_scale_stride=ws.stride(0), y_stride=n, **of_x)
+        whole, required = lib.h3a_linear_fp8_workspace_size(ctypes.byref(args)), lib.h3a_linear_fp8_required_workspace(ctypes.byref(args))
+        assert whole > required and (required == 0) == x8
+        size = required if short else whole
+        room = torch.full((size + 4096,), 91, dtype=torch.uint8, device=DEV)
+        args.workspace, args.workspace_bytes = room.data_ptr(), size
+        assert lib.h3a_linear_fp8(ctypes.byref(args), torch.cuda.current_stream().cuda_stream) == _ext.H3A_OK
+        _check(y[:m], False, q, s, w, ws, None)
+        assert (y[m:] == 7).all() and (room[size:] == 91).all()
+        if not short:
+            assert torch.equal(y[:m], fused_linear_fp8(q, w, ws, x_scale=s))
 
 
 def test_more_than_2_31_values():

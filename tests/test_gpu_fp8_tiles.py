@@ -20,11 +20,12 @@ CASES = [
     (33, 20800, 16, True, False), (33, 4112, 16400, True, False), (1600, 17600, 528, False, True), (33, 17600, 8208, True, False),
     (1000, 144, 1048, False, False), (1000, 144, 1040, False, True), (1000, 144, 536, True, False), (33, 4112, 24, False, False),
     (33, 4112, 16, True, False), (257, 4112, 11200, False, False), (130, 4112, 8208, True, False), (1000, 17600, 2064, False, True),
+    (520, 272, 2072, False, False), (520, 272, 2064, False, True), (520, 272, 1048, True, False),
     (1000, 48, 1048, False, False), (1000, 48, 1040, False, True), (1000, 48, 536, True, False), (97, 8208, 1048, False, False),
     (97, 8208, 528, True, False), (800, 8208, 4800, False, False), (1000, 8208, 2064, True, False), (700, 17600, 4112, False, True),
     # 256 features x 128, 192 and 256 tokens
     (800, 48, 4808, False, False), (800, 48, 4800, False, True), (130, 48, 8208, True, False), (33, 48, 16, True, True), (33, 17600, 16, True, True),
-    (700, 14400, 2064, False, False), (300, 14400, 2072, True, False), (200, 4112, 16400, True, False), (1000, 17600, 4112, False, True),
+    (700, 14400, 2064, False, False), (300, 14400, 4112, False, False), (1000, 11200, 4800, False, False), (390, 11200, 4800, True, False), (300, 14400, 2072, True, False), (200, 4112, 16400, True, False), (1000, 17600, 4112, False, True),
     (1300, 48, 6400, False, False), (1300, 48, 6400, False, True), (130, 48, 16408, True, False), (130, 48, 16400, True, True),
     (130, 14400, 8208, False, False), (130, 14400, 4112, True, False), (1300, 8208, 11200, False, False), (257, 4112, 16400, True, False),
     (520, 17600, 8208, True, False), (130, 17600, 16400, True, True),
