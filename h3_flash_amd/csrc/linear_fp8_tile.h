@@ -53,7 +53,7 @@ __device__ __forceinline__ uint32_t top4(const f32x4& y) {
 // residual, and with a bias alone, the loop has a form of its own. (With a branch per
 // token for each of them, as linear.hip has it, the epilogue took 25,400 of the 129,500
 // cycles of a 256 x 256 tile of k = 5,120, and 32,800 of 140,700 gated, in 8 bits, at
-// k = 5,376.) The tokens' gate rows are looked up once, into LDS behind the rows.
+// k = 5,376; now 9,000 and 16,700.) The tokens' gate rows are looked up once, into LDS behind the rows.
 template <typename T, bool kGated, bool kQuant>
 __device__ __forceinline__ void linear_fp8_epilogue(const LinearFp8Params& p, int f0, int m0, const f32x16 (&acc)[T::NA][T::NB],
                                                     int wn, int wm, int tid, char* smem) {
@@ -223,6 +223,12 @@ __device__ __forceinline__ TileCoord tile_coord(const LinearFp8Params& p, int ti
 
 // Workgroups [0, n_full) run whole tiles, the others the tiles after them in `split`
 // pieces along K, whose sums linear_fp8_join_kernel adds in order (linear.hip).
+// Bound by power where the product is large: 256 x 256 tiles keep the matrix cores 69 to
+// 72% busy at 1.9 to 2.1 GHz. 6,240 x 5,376 x 28,672 gated, into 8 bits: 720 to 775 us on
+// five cards (2,480 to 2,670 TFLOP/s); 6,240 x 14,336 x 5,376 348 to 392, with its 13 last
+// tiles in 8 pieces (whole: 433 to 449); 6,240 x 5,120 x 15,360 376 to 394. Workgroups
+// that stay for several tiles and load the next one's first stages during the epilogue
+// took as long or up to 3% longer, with half the LDS for their epilogue.
 template <int TF, int NT, int SW, int SX, bool kGated, bool kQuant>
 __global__ __launch_bounds__(kPThreads, 1) void linear_fp8_kernel(LinearFp8Params p) {
     using T = Fp8Tile<TF, NT, SW, SX>;
