@@ -4,11 +4,13 @@ tiles, and longer than the scales that a tile holds at once."""
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
-from h3_flash_amd import fused_linear_fp8
-from test_gpu_fp8 import BF16, DEV, F32, _check, _operands, _randn
+from h3_flash_amd import _ext, fused_linear_fp8
+from test_gpu_fp8 import BF16, DEV, E8M0, F32, _check, _operands, _randn
 
 pytestmark = pytest.mark.gpu
 
@@ -57,6 +59,29 @@ def test_rows_after_the_last_are_left_as_they_were():
         out = torch.full((m + 300, 2056), 3.0, dtype=BF16, device=DEV)
         fused_linear_fp8(a, w, w_scale, x_scale=a_scale, out=out[:m])
         assert torch.equal(out[:m], fused_linear_fp8(a, w, w_scale, x_scale=a_scale)) and (out[m:] == 3).all()
+
+
+# (a last tile of one row, of most rows; 256 x 256, 192 and 128 and 128 x 32 tiles)
+@pytest.mark.parametrize("m, k, n, gated", [(1025, 48, 11200, False), (1000, 48, 11200, False), (1345, 48, 6400, False), (257, 48, 16400, True),
+                                            (33, 48, 16, False), (130, 48, 16400, True)])
+@pytest.mark.parametrize("y8", [False, True])
+def test_nothing_behind_a_result_is_written(m, k, n, gated, y8):
+    a, a_scale, w, w_scale = _operands(m, k, n, "fp8", gated)
+    a_scale, w_scale = (torch.nn.functional.pad(s.view(torch.uint8), (0, 16 - s.shape[1])) for s in (a_scale, w_scale))
+    pitch = (n + 127) // 128 // 16 * 16 + 16
+    y = torch.full((m + 300, n if y8 else 2 * n), 91, dtype=torch.uint8, device=DEV)
+    ys = torch.full((m + 300, pitch), 92, dtype=torch.uint8, device=DEV)
+    residual = _randn(m, n, seed=2)
+    args = _ext.LinearFp8Args(
+        abi_version=_ext.ABI_VERSION, x=a.data_ptr(), x_dtype=4, x_scale=a_scale.data_ptr(), weight=w.data_ptr(), weight_scale=w_scale.data_ptr(),
+        residual=residual.data_ptr(), y=y.data_ptr(), y_dtype=4 if y8 else 0, y_scale=ys.data_ptr() if y8 else 0, m=m, k=k, n=n, x_stride=k,
+        x_scale_stride=16, weight_stride=k, weight_scale_stride=16, residual_stride=n, y_stride=n, y_scale_stride=pitch, gated=int(gated))
+    assert _ext.load_library().h3a_linear_fp8(ctypes.byref(args), torch.cuda.current_stream().cuda_stream) == _ext.H3A_OK
+    groups = (n + 127) // 128
+    assert (y[m:] == 91).all() and (ys[m:] == 92).all() and (ys[:, groups:] == 92).all() and (y8 or (ys == 92).all())
+    want = fused_linear_fp8(a, w, w_scale[:, :1].view(E8M0), x_scale=a_scale[:, :1].view(E8M0), gated=gated, residual=residual, quantize=y8)
+    want, scale = want if y8 else (want, None)
+    assert torch.equal(y[:m], want.view(torch.uint8)) and (not y8 or torch.equal(ys[:m, :groups], scale.view(torch.uint8)))
 
 
 @pytest.mark.parametrize("m", [300, 1500])
