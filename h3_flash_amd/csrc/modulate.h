@@ -263,11 +263,17 @@ __global__ __launch_bounds__(kThreads) void modulate_row_kernel(ModulateParams p
         if (k < NV - 1 || last) __builtin_nontemporal_store(ov[kQuant ? 0 : k], (i32x4*)(orow + off[k]));
 }
 
+// The rows up to which the 8-bit forms take a workgroup per row: few rows leave CUs idle,
+// and a row's loads and sum are done the sooner the more waves share it (us, wave /
+// workgroup: 257 x 5,376 6.2 / 3.6, with the residual 8.0 / 4.2; 512 rows 6.6 / 4.5 and 8.5
+// / 6.1, of 1,024 columns 2.9 / 2.7; 1,024 rows 7.0 / 6.0 but with the residual 9.0 / 10.3).
+constexpr int kFewRows = 512;
+
 template <bool kResidual, bool kTabF32, bool kWF32, bool kQuant>
 void launch_modulate_vec(const ModulateParams& p, int nv, hipStream_t stream) {
     const int nw = (int)((p.cols + 511) / 512);  // vectors per lane with one wave per row
     if constexpr (!kTabF32) {
-        if (nw <= kRowVecMax) {
+        if (nw <= kRowVecMax && (!kQuant || p.rows > kFewRows)) {
             const dim3 grid((unsigned)((p.rows + kWaves - 1) / kWaves)), block(kThreads);
             switch (nw) {
 #define H3A_NW(n)                                                                                                     \

@@ -3,7 +3,7 @@
 // they would round it to bf16. Nothing but the row and its scales is written: 3 bytes
 // a value against 7 for a bf16 row and its quantisation (7 against 11 with the
 // residual). 6,240 x 5,376 with the residual: 48 to 50 us for 235 MB, 4.7 to 4.9 TB/s;
-// 257 x 5,376 without: 6.6 us, two dependent rounds of loads and the row's sum.
+// 257 x 5,376 without: 3.6 us, two dependent rounds of loads and the row's sum.
 #include "modulate.h"
 
 namespace h3a {
