@@ -97,9 +97,8 @@ int h3a_quantize_fp8(const h3a_quantize_fp8_args* a, void* stream) {
     if (a->parts < 1 || a->rows % a->parts != 0 || (!blocks && a->parts != 1))
         return fail(H3A_EINVAL, "%s: rows must be `parts` matrices (1 with block_rows 1), got %lld and %lld", fn, (long long)a->rows,
                     (long long)a->parts);
-    // (Work items of a launch: 4 per group, 256 per block.)
     const int64_t scale_rows = blocks ? a->parts * groups_of(a->rows / a->parts) : a->rows;
-    if (a->rows >= ((int64_t)1 << 31) || a->cols >= ((int64_t)1 << 30) || scale_rows * groups_of(a->cols) >= (blocks ? (int64_t)1 << 24 : (int64_t)1 << 30))
+    if (a->rows >= ((int64_t)1 << 31) || a->cols >= ((int64_t)1 << 30) || scale_rows * groups_of(a->cols) > h3a::quantize_max_groups(blocks))
         return fail(H3A_EUNSUPPORTED, "%s: extents too large", fn);
     if (a->rows == 0) return H3A_OK;
     const int64_t size = a->x_dtype == H3A_DTYPE_F32 ? 4 : 2;

@@ -327,6 +327,7 @@ struct QuantizeParams {
     int32_t cols, x_f32, blocks;
 };
 hipError_t launch_quantize(const QuantizeParams& p, hipStream_t stream);
+int64_t quantize_max_groups(bool blocks);  // groups of 128, or blocks, of one launch at most
 
 // The matrix product of 8-bit operands with LinearParams' epilogue; its w, x and y
 // are e4m3 (x: or bf16, rounded to 8 bits first; y: or bf16), all strides in bytes.

@@ -266,7 +266,7 @@ void plan_linear_fp8(LinearFp8Params& p, int cus, int64_t* required, int64_t* wo
     }
     if (p.x_scale == nullptr) {
         *required = rounded_x(p).bytes;
-        if ((int64_t)p.m * ((p.k + kFp8Group - 1) / kFp8Group) >= (int64_t)1 << 30) return;  // as h3a_quantize_fp8
+        if ((int64_t)p.m * ((p.k + kFp8Group - 1) / kFp8Group) > quantize_max_groups(false)) return;
     }
     const int steps = (p.k + kFp8Group - 1) / kFp8Group;
     const float memory_us = kMemoryUs + kMemoryUsPerByte * ((float)w_bytes + (float)p.m * (float)p.k + 2.f * (float)p.m * (float)p.n);

@@ -103,6 +103,8 @@ __global__ __launch_bounds__(kThreads) void quantize_blocks_kernel(QuantizeParam
         if (r + 16 * i < rows) *(i32x2*)((char*)p.q + (row0 + r + 16 * i) * p.q_rs + c) = rounded8<kF32>(raw[i], inv);
 }
 
+constexpr int kRowGroups = 4;  // groups a lane, but for small launches
+
 template <bool kF32>
 void launch_t(const QuantizeParams& p, hipStream_t stream) {
     const int64_t kb = (p.cols + kFp8Group - 1) / kFp8Group;
@@ -114,12 +116,16 @@ void launch_t(const QuantizeParams& p, hipStream_t stream) {
     const int64_t groups = p.rows * kb;
     auto grid = [&](int u) { return dim3((unsigned)((groups + u * (kThreads / 16) - 1) / (u * (kThreads / 16)))); };
     if (groups >= 1 << 16)
-        hipLaunchKernelGGL((quantize_rows_kernel<kF32, 4>), grid(4), dim3(kThreads), 0, stream, p);
+        hipLaunchKernelGGL((quantize_rows_kernel<kF32, kRowGroups>), grid(kRowGroups), dim3(kThreads), 0, stream, p);
     else
         hipLaunchKernelGGL((quantize_rows_kernel<kF32, 1>), grid(1), dim3(kThreads), 0, stream, p);
 }
 
 }  // namespace
+
+// A launch has at most 2^32 - 1 work items, in workgroups of 256: one for each block, or
+// for 64 groups of rows (fewer in the last).
+int64_t quantize_max_groups(bool blocks) { return (int64_t)(UINT32_MAX / kThreads) * (blocks ? 1 : kRowGroups * kThreads / 16); }
 
 hipError_t launch_quantize(const QuantizeParams& p, hipStream_t stream) {
     if (p.rows == 0) return hipSuccess;
