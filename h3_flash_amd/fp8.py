@@ -23,8 +23,7 @@ from __future__ import annotations
 import torch
 
 from . import _ext
-from .fusions import _aligned_rows, _dtype, _empty, _fp8_scales, _index, _index_args, _tables, _vector
-from .linear import _operand
+from .fusions import _aligned_rows, _dtype, _empty, _fp8_scales, _index, _index_args, _operand, _tables, _vector
 
 __all__ = ["fused_linear_fp8", "quantize_fp8", "quantize_fp8_weight"]
 

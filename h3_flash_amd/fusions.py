@@ -119,8 +119,8 @@ def _fp8_scales(lead: tuple[int, ...], columns: int, device: torch.device) -> tu
     return (scale.as_strided((lead[0], groups), (pitch, 1)) if len(lead) == 1 else scale[..., :groups]), pitch
 
 
-def _norm_operand(x: torch.Tensor, name: str, columns: int) -> tuple[torch.Tensor, int, int]:
-    """:func:`_row_span`, of 16-byte aligned rows."""
+def _operand(x: torch.Tensor, name: str, columns: int) -> tuple[torch.Tensor, int, int]:
+    """:func:`_row_span` in rows of 16-byte chunks, as the launch reads them (else a copy)."""
 
     held, rows, stride = _row_span(x, name, columns)
     if stride % 8 or stride < columns or held.data_ptr() % 16:
@@ -269,7 +269,7 @@ def fused_rmsnorm_modulate_fp8(x, weight, scale, shift, index, eps):
 
     columns = x.shape[-1]
     device = x.device
-    held, rows, stride = _norm_operand(x, "x", columns)
+    held, rows, stride = _operand(x, "x", columns)
     weight, tables, index = _norm_fp8_args(weight, [scale, shift], index, columns, device)
     scale, shift = tables
     q = _empty(x.shape, torch.float8_e4m3fn, device)
@@ -291,8 +291,8 @@ def fused_residual_gate_rmsnorm_modulate_fp8(residual, branch, gate, weight, sca
     device = residual.device
     if branch.shape != residual.shape:
         raise ValueError(f"residual {tuple(residual.shape)} and branch {tuple(branch.shape)} differ")
-    rows_r, rows, stride_r = _norm_operand(residual, "residual", columns)
-    rows_b, _, stride_b = _norm_operand(branch, "branch", columns)
+    rows_r, rows, stride_r = _operand(residual, "residual", columns)
+    rows_b, _, stride_b = _operand(branch, "branch", columns)
     if branch.device != device:
         raise ValueError(f"residual and branch must be on one device, got {device} and {branch.device}")
     weight, tables, index = _norm_fp8_args(weight, [gate, scale, shift], index, columns, device)

@@ -15,19 +15,9 @@ from __future__ import annotations
 import torch
 
 from . import _ext
-from .fusions import _aligned_rows, _dtype, _index, _index_args, _row_span, _rows, _tables, _vector
+from .fusions import _aligned_rows, _dtype, _index, _index_args, _operand, _tables, _vector
 
 __all__ = ["fused_linear"]
-
-
-def _operand(x: torch.Tensor, name: str, columns: int) -> tuple[torch.Tensor, int, int]:
-    """Rows of 16-byte chunks: the tensor that holds them, their number and stride."""
-
-    held, rows, stride = _row_span(x, name, columns)
-    if stride % 8 or stride < columns or held.data_ptr() % 16:
-        held = _aligned_rows(_rows(held, name, columns))
-        stride = held.stride(0)
-    return held, rows, stride
 
 
 def fused_linear(
