@@ -14,10 +14,11 @@
 //     no multiplication of their own.) The largest tile's stages leave no LDS for a
 //     ring: there a lane holds its rows' bytes of up to 48 K steps in registers.
 //   - the large tiles read all fragments of an X stage half a K step earlier (kEarlyX).
-// A K step of a 256 x 256 tile takes 2,400 cycles where its MFMAs take 2,048: 70 more
-// between MFMAs on end, 130 at the barrier in the middle, 110 for the fragments' reads,
-// 80 for the scales, the rest for the loads. Of LDS's 128 bytes a cycle it takes three
-// quarters; a wave per SIMD with 128 x 128 of the result is what keeps it there.
+// A K step of a 256 x 256 tile takes 2,400 cycles where its MFMAs take 2,048; the others
+// are gaps between MFMAs on end, the barriers, and MFMAs held up by the fragments' reads,
+// the scales and the loads, which overlap. It writes 64 KB to LDS and reads 128: at 128
+// bytes a cycle 1,536 cycles, three quarters of the MFMAs' and 64% of the step's. A wave
+// per SIMD with 128 x 128 of the result is what keeps it there.
 #pragma once
 
 #include "gemm_tile.h"

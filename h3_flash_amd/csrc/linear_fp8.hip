@@ -33,7 +33,7 @@ constexpr int kRowsMaxTokens = 32;
 // by the tiles' deep rings of loads, also for one block of 16 tokens and a launch more
 // that rounds bf16 rows (us, this form at its best / tiles: 16 x 5,376 x 5,376 12.4 /
 // 14.7; 16 x 14,336 x 5,376 26.2 / 20.4; 16 x 5,376 x 32,256 37.2 / 31.5; 32 x 1,024 x
-// 4,096 5.4 / 6.4; 32 x 5,376 x 5,376 16.8 / 15).
+// 4,096 5.4 / 6.4; 32 x 5,376 x 5,376 16.8 / 15: the limits lie between those points).
 constexpr int64_t kRowsMaxWeight[2] = {48 << 20, 16 << 20};  // bytes, up to 16 and 32 tokens
 constexpr int kRowsForm = -1, kNoForm = -2;  // in place of a tile shape
 
@@ -289,7 +289,9 @@ void plan_linear_fp8(LinearFp8Params& p, int cus, int64_t* required, int64_t* wo
         int split = 1;
         // The last round in pieces, at most one per CU (of the smallest tiles none: they
         // serve short reductions; nor with the result in 8 bits, whose groups the join's
-        // workgroups do not hold).
+        // workgroups, 32 tokens x 8 features a wave, do not hold: with few tiles over a long
+        // reduction that costs up to four times a bf16 result's time, 64 x 14,336 x 1,024
+        // gated 65.8 us against 15.1, 256 x 5,376 x 2,688 29.8 against 20.8).
         for (const int n : kSplits) {
             if (rest == 0 || rest * n > cus || steps / n < kMinPieceSteps || s.nt == 2 || p.y_scale != nullptr) break;
             const float cut = (float)(full / cus) * tile_us + last_us(n) + kJoinUs + (float)(rest * n * s.tf * tokens * 4) * kJoinUsPerByte;

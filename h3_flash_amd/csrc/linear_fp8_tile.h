@@ -224,11 +224,12 @@ __device__ __forceinline__ TileCoord tile_coord(const LinearFp8Params& p, int ti
 // Workgroups [0, n_full) run whole tiles, the others the tiles after them in `split`
 // pieces along K, whose sums linear_fp8_join_kernel adds in order (linear.hip).
 // Bound by power where the product is large: 256 x 256 tiles keep the matrix cores 69 to
-// 72% busy at 1.9 to 2.1 GHz. 6,240 x 5,376 x 28,672 gated, into 8 bits: 718 to 782 us on
-// six cards (2,460 to 2,680 TFLOP/s); 6,240 x 14,336 x 5,376 348 to 392, with its 13 last
-// tiles in 8 pieces (whole: 433 to 449); 6,240 x 5,120 x 15,360 376 to 394. Workgroups
-// that stay for several tiles and load the next one's first stages during the epilogue
-// took as long or up to 3% longer, with half the LDS for their epilogue.
+// 72% busy at 1.9 to 2.1 GHz. In graph replays on seven cards 6,240 x 5,376 x 28,672 gated,
+// into 8 bits, takes 717 to 782 us (2,460 to 2,680 TFLOP/s), 6,240 x 14,336 x 5,376 348 to
+// 378, with its 13 last tiles in 8 pieces (whole: 433 to 449), 6,240 x 5,120 x 15,360 from
+// 8-bit rows 376 to 398. Workgroups that stay for several tiles and load the next one's
+// first stages during the epilogue took as long or up to 3% longer, with half the LDS for
+// their epilogue.
 template <int TF, int NT, int SW, int SX, bool kGated, bool kQuant>
 __global__ __launch_bounds__(kPThreads, 1) void linear_fp8_kernel(LinearFp8Params p) {
     using T = Fp8Tile<TF, NT, SW, SX>;

@@ -267,6 +267,7 @@ __global__ __launch_bounds__(kThreads) void modulate_row_kernel(ModulateParams p
 // and a row's loads and sum are done the sooner the more waves share it (us, wave /
 // workgroup: 257 x 5,376 6.2 / 3.6, with the residual 8.0 / 4.2; 512 rows 6.6 / 4.5 and 8.5
 // / 6.1, of 1,024 columns 2.9 / 2.7; 1,024 rows 7.0 / 6.0 but with the residual 9.0 / 10.3).
+// One limit for both: the residual's; without it a workgroup still gains 1 us at 1,024 rows.
 constexpr int kFewRows = 512;
 
 template <bool kResidual, bool kTabF32, bool kWF32, bool kQuant>
